@@ -216,16 +216,16 @@ def _run_label_probs(state):
     k, T = case["topk"], case["temperature"]
     if own:
         ops = _framework()[0]
-        kw = dict(temperature=T, ignore_label=IGNORE, class_mask=mask)
-        out = ops.native.label_log_probs(logits, labels, topk=k, want_stats=case["backward"], **kw)
+        out = ops.native.label_log_probs(logits, labels, topk=k, temperature=T, ignore_label=IGNORE, class_mask=mask,
+                                         want_stats=case["backward"])
         got = {"entropy": out.entropy}
         if labels is not None:
             got["log_prob"] = out.log_prob
         if k:
             got.update(top_ids=out.top_ids, top_log_probs=out.top_log_probs)
         if case["backward"]:
-            got["d_logits"] = ops.native.label_log_probs_bwd(logits, labels, out.stats, state["d_log_prob"],
-                                                             state.get("d_entropy"), **kw)
+            got["d_logits"] = ops.native.label_log_probs_bwd(logits, out.stats, state["d_log_prob"],
+                                                             state.get("d_entropy"), temperature=T, class_mask=mask)
         return got
     x = logits.float()
     if mask is not None:
