@@ -35,6 +35,7 @@ enum {
   LDM_ERR_ARG = 1,     /* bad argument / unsupported configuration */
   LDM_ERR_ALIGN = 2,   /* pointer or channel count violates the vector-width requirement */
   LDM_ERR_LAUNCH = 3,  /* hipLaunchKernel failed */
+  LDM_ERR_OVERLAP = 4, /* operands that a call writes overlap in memory */
 };
 
 /* ---------------------------------------------------------------------------------------
@@ -709,6 +710,79 @@ size_t ldm_reduce_workspace_bytes(void);
 int ldm_adamw(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, const void* segments, int nseg,
               int64_t n, float beta1, float beta2, float eps, int step, const double* sqsum, float max_norm,
               ldm_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * ldm_label_log_probs — per position: log probability of a given label, entropy and the k most
+ * likely classes of softmax(logits / temperature); ldm_label_log_probs_bwd — its gradient.
+ *
+ * A position is (i0, i1, i2) < (n0, n1, n2); class c of it is logits[i0*s0 + i1*s1 + i2*s2 + c*sc]
+ * (elements, any non-negative strides), dtype LDM_F32 / LDM_BF16, arithmetic in fp32.  All other
+ * arrays are contiguous over the positions, i2 fastest.
+ *   labels       int64 or NULL.  label == ignore_label (with has_ignore): log_prob 0; outside
+ *                [0, classes): log_prob NaN; a class without probability: log_prob -inf.
+ *   class_mask   bytes or NULL: classes with 0 are left out, whatever their logits hold (NaN and
+ *                infinities included); position p uses mask + (p / mask_div) * mask_stride.
+ *   topk         0..LDM_LABEL_TOPK_MAX, <= classes.  Larger logit first, ties: lower class first;
+ *                top_ids -1 / top_log_probs -inf past the classes with probability.  Entry j of
+ *                position p is at (p / inner) * topk * inner + j * inner + p % inner.
+ *   stats        NULL, or fp32 [4][positions] for the backward: max logit, log of the sum,
+ *                entropy, label (int32 bits; -1: no gradient through log_prob).
+ * A row with no class left (all masked or -inf): entropy 0, ids -1.  NaN or +inf among the
+ * classes left: log_prob and entropy NaN.  temperature in [1e-4, 1e4].
+ * ldm_label_log_probs_bwd: d_logits = (d_log_prob * (onehot(label) - p) - d_entropy * p * (log p +
+ * entropy)) / temperature, written at the out strides o0, o1, o2, oc (the row's masked classes and
+ * empty rows: 0). d_log_prob / d_entropy fp32 over the positions, either may be NULL. */
+#define LDM_LABEL_TOPK_MAX 16
+typedef struct {
+  const void* logits;
+  int64_t n0, n1, n2, s0, s1, s2, classes, sc;
+  const int64_t* labels;
+  int64_t ignore_label;
+  const void* class_mask;
+  int64_t mask_stride, mask_div, inner;
+  float* log_prob;
+  float* entropy;
+  float* top_log_probs;
+  int32_t* top_ids;
+  float* stats;
+  void* workspace;
+  int64_t workspace_bytes;
+  float temperature;
+  int has_ignore, topk, dtype;
+} ldm_label_probs_params;
+typedef struct {
+  const void* logits;
+  int64_t n0, n1, n2, s0, s1, s2, classes, sc;
+  const void* class_mask;
+  int64_t mask_stride, mask_div;
+  const float* stats;
+  const float* d_log_prob;
+  const float* d_entropy;
+  void* d_logits;
+  int64_t o0, o1, o2, oc;
+  float temperature;
+  int dtype;
+} ldm_label_probs_bwd_params;
+size_t ldm_label_log_probs_workspace_bytes(const ldm_label_probs_params* p);
+int ldm_label_log_probs(const ldm_label_probs_params* p, ldm_stream_t stream);
+int ldm_label_log_probs_bwd(const ldm_label_probs_bwd_params* p, ldm_stream_t stream);
+
+/* ldm_grad_norm — the global norm of many gradient tensors, and clipping them in place.
+ *   ptrs, numel, dtypes   HOST arrays of ntensors device pointers, element counts and dtype codes
+ *                         (LDM_F32 / LDM_BF16, mixed freely); each tensor is dense memory, aligned
+ *                         to its element; tensors must not overlap (LDM_ERR_OVERLAP).  The arrays are
+ *                         read during the call only: a captured graph keeps its own copy.
+ *   norm_type             LDM_NORM_2 (sqrt of the fp64 sum of squares), LDM_NORM_INF, LDM_NORM_1
+ *   out                   device fp32 [2]: the norm and the factor min(1, max_norm / (norm + 1e-6))
+ *   clip                  0: norm only.  1: norm, then every g *= factor where the factor is below
+ *                         1 or NaN (torch.nn.utils.clip_grad_norm_'s arithmetic).  2: only the
+ *                         scaling, by the factor already in out
+ * Sums run in a fixed order (no atomics): the same gradients give the same bits. */
+enum { LDM_NORM_2 = 0, LDM_NORM_INF = 1, LDM_NORM_1 = 2 };
+size_t ldm_grad_norm_workspace_bytes(const int64_t* numel, int ntensors);
+int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, const uint8_t* dtypes, int ntensors, int norm_type,
+                  double max_norm, int clip, float* out, void* workspace, int64_t workspace_bytes,
+                  ldm_stream_t stream);
 
 const char* ldm_status_string(int status);
 int ldm_abi_version(void);

@@ -1,0 +1,201 @@
+// Global gradient norm over many tensors, and clipping them in place (ldm_grad_norm).
+//
+//   norm   = sqrt(sum g^2), max |g| or sum |g| over every element of every tensor
+//   factor = min(1, max_norm / (norm + 1e-6));  g *= factor   (torch.nn.utils.clip_grad_norm_)
+// The tensors' addresses travel as kernel arguments, up to TABLE of them to a launch: nothing is
+// copied to the device, nothing is kept between calls, and a captured graph holds its own table.
+// Squares are summed in fp64 (a square of any fp32 value is finite there), per thread, block and
+// partial in a fixed order: the same gradients give the same bits.
+#include "common.h"
+
+#include <algorithm>
+#include <math.h>
+#include <vector>
+
+namespace {
+
+constexpr int TABLE = 224;               // tensors to a launch: 16 B each, below the 4 KB of kernel arguments
+constexpr int CHUNK = 8192;              // elements a block takes at a time
+constexpr int MAX_BLOCKS = 2048;
+
+struct Entry {
+  uint64_t ptr;                          // bit 63: bf16
+  uint32_t n, chunk0;                    // elements, first chunk
+};
+struct Table {
+  Entry e[TABLE];
+  int count, chunks;
+};
+
+__device__ __forceinline__ int entry_of(const Table& t, int chunk) {   // the last entry with chunk0 <= chunk
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((int)t.e[mid].chunk0 <= chunk) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <int NORM> __device__ __forceinline__ double norm_add(double acc, float g) {
+  if (NORM == LDM_NORM_2) return fma((double)g, (double)g, acc);
+  if (NORM == LDM_NORM_1) return acc + fabs((double)g);
+  const double a = fabs((double)g);
+  return (a > acc || a != a) ? a : acc;          // a NaN stays
+}
+template <int NORM> __device__ __forceinline__ double norm_join(double a, double b) {
+  if (NORM != LDM_NORM_INF) return a + b;
+  return (b > a || b != b) ? b : a;
+}
+template <int NORM> __device__ __forceinline__ double block_join(double v) {
+  __shared__ double part[4];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = norm_join<NORM>(v, __shfl_xor(v, o, 64));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return norm_join<NORM>(norm_join<NORM>(part[0], part[1]), norm_join<NORM>(part[2], part[3]));
+}
+
+template <int NORM, typename T>
+__device__ __forceinline__ double chunk_norm(const T* g, int64_t n, double acc) {
+  for (int64_t i = threadIdx.x; i < n; i += 256) acc = norm_add<NORM>(acc, to_f(g[i]));
+  return acc;
+}
+
+template <int NORM>
+__global__ __launch_bounds__(256) void norm_parts(const Table t, double* __restrict__ part) {
+  double acc = 0.0;
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const Entry e = t.e[entry_of(t, c)];
+    const int64_t at = (int64_t)(c - (int)e.chunk0) * CHUNK;
+    const int64_t n = min((int64_t)CHUNK, (int64_t)e.n - at);
+    if (e.ptr >> 63) acc = chunk_norm<NORM>((const bf16_t*)(e.ptr & ~(1ull << 63)) + at, n, acc);
+    else acc = chunk_norm<NORM>((const float*)e.ptr + at, n, acc);
+  }
+  acc = block_join<NORM>(acc);
+  if (threadIdx.x == 0) part[blockIdx.x] = acc;
+}
+
+// min(1, max / (norm + 1e-6)) with a NaN kept, in fp32 from the rounded norm
+__device__ __forceinline__ float factor_of(float norm, float max_norm) {
+  const float f = max_norm / (norm + 1e-6f);
+  return f > 1.f ? 1.f : f;
+}
+
+template <int NORM>
+__global__ __launch_bounds__(256) void norm_final(const double* __restrict__ part, int parts, float max_norm,
+                                                  float* __restrict__ out) {
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < parts; i += 256) acc = norm_join<NORM>(acc, part[i]);
+  acc = block_join<NORM>(acc);
+  if (threadIdx.x == 0) {
+    out[0] = (float)(NORM == LDM_NORM_2 ? sqrt(acc) : acc);
+    out[1] = factor_of(out[0], max_norm);
+  }
+}
+
+// a gradient is multiplied by the factor as its own type holds it and rounded once, as torch's in-place product
+// of a tensor with a device scalar is: a bf16 gradient's factor has 8 bits
+template <typename T>
+__device__ __forceinline__ void chunk_scale(T* g, int64_t n, float factor) {
+  const float f = to_f(from_f<T>(factor));
+  if (f == 1.f) return;
+  for (int64_t i = threadIdx.x; i < n; i += 256) g[i] = from_f<T>(to_f(g[i]) * f);
+}
+
+__global__ __launch_bounds__(256) void scale_all(const Table t, const float* __restrict__ out) {
+  const float f = out[1];
+  if (f == 1.f) return;
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const Entry e = t.e[entry_of(t, c)];
+    const int64_t at = (int64_t)(c - (int)e.chunk0) * CHUNK;
+    const int64_t n = min((int64_t)CHUNK, (int64_t)e.n - at);
+    if (e.ptr >> 63) chunk_scale((bf16_t*)(e.ptr & ~(1ull << 63)) + at, n, f);
+    else chunk_scale((float*)e.ptr + at, n, f);
+  }
+}
+
+// a tensor above 2^30 elements is listed in pieces
+constexpr int64_t PIECE = 1LL << 30;
+int64_t entries_of(const int64_t* numel, int n) {
+  int64_t c = 0;
+  for (int i = 0; i < n; ++i) c += (numel[i] + PIECE - 1) / PIECE;
+  return c;
+}
+
+template <int NORM>
+void launch_norm(const Table& t, int blocks, double* part, hipStream_t s) {
+  hipLaunchKernelGGL((norm_parts<NORM>), dim3(blocks), dim3(256), 0, s, t, part);
+}
+
+}  // namespace
+
+extern "C" size_t ldm_grad_norm_workspace_bytes(const int64_t* numel, int ntensors) {
+  if (!numel || ntensors <= 0) return 0;
+  return (size_t)((entries_of(numel, ntensors) + TABLE - 1) / TABLE) * MAX_BLOCKS * sizeof(double);
+}
+
+extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, const uint8_t* dtypes, int ntensors,
+                             int norm_type, double max_norm, int clip, float* out, void* workspace,
+                             int64_t workspace_bytes, ldm_stream_t stream) {
+  if (!ptrs || !numel || !dtypes || !out || ntensors <= 0 || clip < 0 || clip > 2) return LDM_ERR_ARG;
+  if (norm_type < LDM_NORM_2 || norm_type > LDM_NORM_1 || !(max_norm >= 0.0)) return LDM_ERR_ARG;
+  const int64_t need = clip == 2 ? 0 : (int64_t)ldm_grad_norm_workspace_bytes(numel, ntensors);
+  if (need && (!workspace || workspace_bytes < need)) return LDM_ERR_ARG;
+  struct Span { uint64_t lo, hi; };
+  std::vector<Span> spans;
+  std::vector<Table> tables;
+  try {
+    spans.reserve(ntensors);
+    for (int i = 0; i < ntensors; ++i) {
+      if (numel[i] < 0 || dtypes[i] > LDM_BF16) return LDM_ERR_ARG;
+      if (numel[i] == 0) continue;
+      const uint64_t a = reinterpret_cast<uint64_t>(ptrs[i]);
+      const uint64_t size = dtypes[i] == LDM_BF16 ? 2 : 4;
+      if (!a || (a >> 63)) return LDM_ERR_ARG;
+      if (a % size) return LDM_ERR_ALIGN;
+      spans.push_back({a, a + size * (uint64_t)numel[i]});
+      for (int64_t at = 0; at < numel[i]; at += PIECE) {
+        if (tables.empty() || tables.back().count == TABLE) {
+          tables.emplace_back();
+          tables.back().count = tables.back().chunks = 0;
+        }
+        Table& t = tables.back();
+        const int64_t n = std::min(PIECE, numel[i] - at);
+        t.e[t.count++] = {(a + size * (uint64_t)at) | ((uint64_t)(dtypes[i] == LDM_BF16) << 63), (uint32_t)n,
+                          (uint32_t)t.chunks};
+        t.chunks += (int)((n + CHUNK - 1) / CHUNK);
+      }
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span& p, const Span& q) { return p.lo < q.lo; });
+  } catch (...) {
+    return LDM_ERR_ARG;
+  }
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].lo < spans[i - 1].hi) return LDM_ERR_OVERLAP;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  double* part = static_cast<double*>(workspace);
+  if (clip != 2) {
+    int parts = 0;
+    for (const Table& t : tables) {
+      const int blocks = std::min(t.chunks, MAX_BLOCKS);
+      if (norm_type == LDM_NORM_2) launch_norm<LDM_NORM_2>(t, blocks, part + parts, s);
+      else if (norm_type == LDM_NORM_INF) launch_norm<LDM_NORM_INF>(t, blocks, part + parts, s);
+      else launch_norm<LDM_NORM_1>(t, blocks, part + parts, s);
+      LDM_CHECK_LAUNCH();
+      parts += blocks;
+    }
+    if (norm_type == LDM_NORM_2)
+      hipLaunchKernelGGL((norm_final<LDM_NORM_2>), dim3(1), dim3(256), 0, s, part, parts, (float)max_norm, out);
+    else if (norm_type == LDM_NORM_INF)
+      hipLaunchKernelGGL((norm_final<LDM_NORM_INF>), dim3(1), dim3(256), 0, s, part, parts, (float)max_norm, out);
+    else
+      hipLaunchKernelGGL((norm_final<LDM_NORM_1>), dim3(1), dim3(256), 0, s, part, parts, (float)max_norm, out);
+    LDM_CHECK_LAUNCH();
+  }
+  if (clip)
+    for (const Table& t : tables) {
+      hipLaunchKernelGGL(scale_all, dim3(std::min(t.chunks, MAX_BLOCKS)), dim3(256), 0, s, t, out);
+      LDM_CHECK_LAUNCH();
+    }
+  return LDM_OK;
+}

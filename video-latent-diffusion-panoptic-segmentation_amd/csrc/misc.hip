@@ -393,6 +393,7 @@ extern "C" const char* ldm_status_string(int status) {
     case LDM_ERR_ARG: return "invalid argument or unsupported configuration";
     case LDM_ERR_ALIGN: return "pointer / channel alignment violates the 16-byte vector requirement";
     case LDM_ERR_LAUNCH: return "kernel launch failed";
+    case LDM_ERR_OVERLAP: return "operands overlap in memory";
     default: return "unknown status";
   }
 }

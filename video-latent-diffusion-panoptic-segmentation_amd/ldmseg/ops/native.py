@@ -5,6 +5,8 @@ no fallback: if the library is missing, or a tensor is not on the GPU, the call 
 Host-side checks (device, dtype, contiguity, shapes) run before any launch so that a bad
 call can never reach the GPU as an out-of-bounds kernel.
 """
+import array
+import collections
 import contextlib
 import ctypes
 import math
@@ -17,6 +19,7 @@ PKG_ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__fil
 LIB_PATH = os.path.join(PKG_ROOT, "lib", "libldmseg_hip.so")
 
 F32, BF16 = 0, 1
+ERR_OVERLAP = 4
 OUT_NHWC, OUT_NCHW, OUT_GEGLU, OUT_SHUFFLE2 = 0, 1, 2, 3
 ACT_NONE, ACT_SILU, ACT_RELU, ACT_SIGMOID = 0, 1, 2, 3
 PRED = {"epsilon": 0, "sample": 1, "v_prediction": 2}
@@ -79,6 +82,21 @@ class DdimParams(ctypes.Structure):
                 ("x0", _vp), ("out_dtype", _i), ("n", _i64), ("t", _vp), ("alphas_cumprod", _vp),
                 ("final_alpha_cumprod", _f), ("step_ratio", _i), ("prediction_type", _i), ("clip_sample", _i),
                 ("clip_range", _f), ("use_clipped_model_output", _i), ("num_train_timesteps", _i)]
+
+
+class LabelProbsParams(ctypes.Structure):
+    _fields_ = [("logits", _vp), ("n0", _i64), ("n1", _i64), ("n2", _i64), ("s0", _i64), ("s1", _i64), ("s2", _i64),
+                ("classes", _i64), ("sc", _i64), ("labels", _vp), ("ignore_label", _i64), ("class_mask", _vp),
+                ("mask_stride", _i64), ("mask_div", _i64), ("inner", _i64), ("log_prob", _vp), ("entropy", _vp),
+                ("top_log_probs", _vp), ("top_ids", _vp), ("stats", _vp), ("workspace", _vp),
+                ("workspace_bytes", _i64), ("temperature", _f), ("has_ignore", _i), ("topk", _i), ("dtype", _i)]
+
+
+class LabelProbsBwdParams(ctypes.Structure):
+    _fields_ = [("logits", _vp), ("n0", _i64), ("n1", _i64), ("n2", _i64), ("s0", _i64), ("s1", _i64), ("s2", _i64),
+                ("classes", _i64), ("sc", _i64), ("class_mask", _vp), ("mask_stride", _i64), ("mask_div", _i64),
+                ("stats", _vp), ("d_log_prob", _vp), ("d_entropy", _vp), ("d_logits", _vp), ("o0", _i64),
+                ("o1", _i64), ("o2", _i64), ("oc", _i64), ("temperature", _f), ("dtype", _i)]
 
 
 EXPORTS = {
@@ -175,6 +193,11 @@ EXPORTS = {
     "ldm_space_to_depth2": (_i, [_vp, _i, _i, _i, _i, _vp, _i, _vp]),
     "ldm_posterior_sample": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp]),
     "ldm_posterior_bwd": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
+    "ldm_label_log_probs_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LabelProbsParams)]),
+    "ldm_label_log_probs": (_i, [ctypes.POINTER(LabelProbsParams), _vp]),
+    "ldm_label_log_probs_bwd": (_i, [ctypes.POINTER(LabelProbsBwdParams), _vp]),
+    "ldm_grad_norm_workspace_bytes": (ctypes.c_size_t, [_vp, _i]),
+    "ldm_grad_norm": (_i, [_vp, _vp, _vp, _i, _i, _d, _i, _vp, _vp, _i64, _vp]),
     "ldm_status_string": (ctypes.c_char_p, [_i]),
     "ldm_abi_version": (_i, []),
 }
@@ -234,6 +257,14 @@ def _gpu(*ts):
 
 def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(dev):
+    """Context in which launches go to ``dev`` (nothing to do where it is the current device)."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _contig(t, name):
@@ -1837,3 +1868,252 @@ def posterior_bwd(moments, eps, dz_nhwc):
     _check(lib.ldm_posterior_bwd(_ptr(moments), _ptr(eps), _ptr(dz_nhwc), cs, B, C2 // 2, H * W, _ptr(dm),
                                  dtype_code(dz_nhwc.dtype), _stream(moments)), "ldm_posterior_bwd")
     return dm
+
+
+# ======================================================================================
+# label probabilities: log probability of a given label, entropy, most likely alternatives
+# ======================================================================================
+LABEL_TOPK_MAX = 16
+LabelProbs = collections.namedtuple("LabelProbs", "log_prob entropy top_log_probs top_ids stats")
+
+
+def _merge_dims(sizes, *strides):
+    """(sizes, strides...) without dims of size 1 and with adjacent dims merged where every layout has them
+    one stride apart."""
+    ns, out = [], [[] for _ in strides]
+    for i, n in enumerate(sizes):
+        if n == 1:
+            continue
+        if ns and all(o[-1] == n * s[i] for o, s in zip(out, strides)):
+            ns[-1] *= n
+            for o, s in zip(out, strides):
+                o[-1] = s[i]
+        else:
+            ns.append(n)
+            for o, s in zip(out, strides):
+                o.append(s[i])
+    return ns, out
+
+
+def _label_positions(x, dim, grad=False):
+    """The positions of ``x`` (every dim but ``dim``) as up to three strided dims: (x, sizes, strides,
+    n_positions, inner, out, out strides).  ``inner`` counts the positions behind the class dim; dims are
+    merged on either side of it, never across it, and a tensor with more than three left is copied.  With
+    ``grad``, ``out`` is an uninitialised tensor like x, walked by the same sizes."""
+    if x.is_contiguous():
+        inner = math.prod(x.shape[dim + 1:])
+        outer = math.prod(x.shape[:dim])
+        s = (0, x.shape[dim] * inner, 1)
+        return x, (1, outer, inner), s, outer * inner, inner, torch.empty_like(x) if grad else None, s
+    out = torch.empty_like(x) if grad else None
+    layouts = [x.stride()] + ([out.stride()] if grad else [])
+    no, so = _merge_dims(x.shape[:dim], *[st[:dim] for st in layouts])
+    ni, si = _merge_dims(x.shape[dim + 1:], *[st[dim + 1:] for st in layouts])
+    n = no + ni
+    if len(n) > 3:
+        return _label_positions(x.contiguous(), dim, grad)
+    pad = 3 - len(n)
+    s = [[0] * pad + a + b for a, b in zip(so, si)]
+    return x, [1] * pad + n, s[0], math.prod(n), math.prod(ni), out, s[-1]
+
+
+def _label_mask(class_mask, logits, dim, n_positions):
+    """(mask, row stride, positions to a row) of a class mask [C] or [logits.shape[0], C]."""
+    if class_mask is None:
+        return None, 0, 1
+    C, B = logits.shape[dim], logits.shape[0]
+    if class_mask.dtype != torch.bool or class_mask.device != logits.device:
+        raise TypeError("class_mask must be a bool tensor on the logits' device")
+    if tuple(class_mask.shape) == (C,):
+        return class_mask.contiguous(), 0, max(1, n_positions)
+    if dim != 0 and tuple(class_mask.shape) == (B, C):
+        return class_mask.contiguous(), C, max(1, n_positions // max(1, B))
+    raise ValueError(f"class_mask must be [{C}] or [{B}, {C}] (classes, or the logits' first dim by classes), got "
+                     f"{tuple(class_mask.shape)}")
+
+
+def _label_dim(logits, dim):
+    if logits.ndim < 2:
+        raise ValueError("logits need a class dim and at least one position dim")
+    d = dim + logits.ndim if dim < 0 else dim
+    if not 0 <= d < logits.ndim:
+        raise ValueError(f"class dim {dim} is outside logits of {logits.ndim} dims")
+    if logits.shape[d] == 0:
+        raise ValueError("logits have no classes")
+    return d
+
+
+def _label_temperature(t):
+    if not 1e-4 <= t <= 1e4:
+        raise ValueError(f"temperature must be in [1e-4, 1e4], got {t}")
+    return float(t)
+
+
+def label_log_probs(logits, labels=None, *, dim=1, topk=0, temperature=1.0, ignore_label=None, class_mask=None,
+                    want_stats=False):
+    """Per position of ``logits`` (fp32 / bf16, any strides, classes along ``dim``), in one pass over them,
+    of softmax(logits / temperature):
+
+      log_prob       fp32 [positions]: log probability of ``labels`` (int64, the logits' shape without
+                     ``dim``); 0 where a label is ``ignore_label``, NaN where it is no class, -inf where
+                     its class has no probability.  None without labels
+      entropy        fp32 [positions], in nats
+      top_log_probs  fp32, the logits' shape with ``topk`` (<= 16) in place of the classes: the most likely
+      top_ids        int32 alternatives, larger logit first, then lower class; -inf / -1 behind the classes
+                     that have probability.  None without topk
+      stats          fp32 [4, positions...] for label_log_probs_bwd (``want_stats``)
+
+    ``class_mask`` (bool [C] or [logits.shape[0], C]) leaves classes out whatever their logits hold.  A row
+    that is left without a class has entropy 0 and no alternatives; a NaN or +inf among the classes left
+    makes the row's log_prob and entropy NaN."""
+    code = dtype_code(logits.dtype)
+    dim = _label_dim(logits, dim)
+    temperature = _label_temperature(temperature)
+    shape = logits.shape
+    C = shape[dim]
+    pos_shape = shape[:dim] + shape[dim + 1:]
+    if not 0 <= topk <= min(C, LABEL_TOPK_MAX):
+        raise ValueError(f"topk must be in [0, {min(C, LABEL_TOPK_MAX)}], got {topk}")
+    dev = logits.device
+    if labels is not None:
+        if labels.dtype != torch.int64 or labels.device != dev:
+            raise TypeError("labels must be an int64 tensor on the logits' device")
+        if labels.shape != pos_shape:
+            raise ValueError(f"labels must be {tuple(pos_shape)}, got {tuple(labels.shape)}")
+        labels = labels.contiguous()
+    N = math.prod(pos_shape)
+    mask, mask_stride, mask_div = _label_mask(class_mask, logits, dim, N)
+    _gpu(logits)
+    lib = load_library()
+    x, n, s, _, inner, _, _ = _label_positions(logits, dim)
+    entropy = torch.empty(pos_shape, dtype=torch.float32, device=dev)
+    log_prob = None if labels is None else torch.empty_like(entropy)
+    top_lp = top_id = stats = None
+    if topk:
+        top_shape = shape[:dim] + (topk,) + shape[dim + 1:]
+        top_lp = torch.empty(top_shape, dtype=torch.float32, device=dev)
+        top_id = torch.empty(top_shape, dtype=torch.int32, device=dev)
+    if want_stats:
+        stats = torch.empty((4,) + pos_shape, dtype=torch.float32, device=dev)
+    if N:
+        p = LabelProbsParams(x.data_ptr(), *n, *s, C, x.stride(dim), _ptr(labels),
+                             0 if ignore_label is None else int(ignore_label), _ptr(mask), mask_stride, mask_div,
+                             inner, _ptr(log_prob), entropy.data_ptr(), _ptr(top_lp), _ptr(top_id), _ptr(stats), None,
+                             0, temperature, ignore_label is not None, topk, code)
+        with _on_device(dev):
+            ref = ctypes.byref(p)
+            wsb = lib.ldm_label_log_probs_workspace_bytes(ref)
+            if wsb:
+                ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+                p.workspace, p.workspace_bytes = ws.data_ptr(), wsb
+            _check(lib.ldm_label_log_probs(ref, _stream(logits)), "ldm_label_log_probs")
+    return LabelProbs(log_prob, entropy, top_lp, top_id, stats)
+
+
+def _upstream(g, shape, dev, name):
+    if g is None:
+        return None
+    if g.dtype != torch.float32 or g.device != dev or g.shape != shape:
+        raise ValueError(f"{name} must be fp32 {tuple(shape)} on the logits' device")
+    return g.contiguous()
+
+
+def label_log_probs_bwd(logits, stats, d_log_prob=None, d_entropy=None, *, dim=1, temperature=1.0, class_mask=None):
+    """The logits' gradient (their shape, type and layout) from the gradients of label_log_probs' log_prob and
+    entropy (fp32 [positions], either may be None), its ``stats`` and its other arguments.  Masked classes,
+    rows without a class and log_prob of ignored, invalid or impossible labels get none."""
+    code = dtype_code(logits.dtype)
+    dim = _label_dim(logits, dim)
+    temperature = _label_temperature(temperature)
+    pos_shape = logits.shape[:dim] + logits.shape[dim + 1:]
+    dev = logits.device
+    if stats.dtype != torch.float32 or stats.device != dev or stats.shape != (4,) + pos_shape \
+            or not stats.is_contiguous():
+        raise ValueError(f"stats must be label_log_probs' fp32 {(4,) + tuple(pos_shape)}")
+    gl = _upstream(d_log_prob, pos_shape, dev, "d_log_prob")
+    ge = _upstream(d_entropy, pos_shape, dev, "d_entropy")
+    N = math.prod(pos_shape)
+    mask, mask_stride, mask_div = _label_mask(class_mask, logits, dim, N)
+    _gpu(logits)
+    lib = load_library()
+    x, n, s, _, _, out, o = _label_positions(logits, dim, grad=True)
+    if N:
+        p = LabelProbsBwdParams(x.data_ptr(), *n, *s, x.shape[dim], x.stride(dim), _ptr(mask), mask_stride, mask_div,
+                                stats.data_ptr(), _ptr(gl), _ptr(ge), out.data_ptr(), *o, out.stride(dim), temperature,
+                                code)
+        with _on_device(dev):
+            _check(lib.ldm_label_log_probs_bwd(ctypes.byref(p), _stream(logits)), "ldm_label_log_probs_bwd")
+    return out
+
+
+# ======================================================================================
+# global gradient norm over many tensors, and clipping
+# ======================================================================================
+NORM_TYPES = {2.0: 0, math.inf: 1, 1.0: 2}
+
+
+def _grad_arrays(grads):
+    """Host arrays (addresses, element counts, dtype codes) of dense gradients on one GPU, and their device."""
+    dev = grads[0].device
+    try:
+        codes = bytes([_GRAD_CODES[g.dtype] for g in grads])
+    except KeyError as e:
+        raise TypeError(f"unsupported gradient dtype {e.args[0]}: float32 or bfloat16") from None
+    for g in grads:
+        if g.device != dev:
+            raise ValueError(f"gradients on {dev} and {g.device}: one device per call")
+        if g.layout != torch.strided:
+            raise TypeError("sparse gradients are not supported")
+        if not g.is_contiguous() and not _is_dense(g):
+            raise ValueError("a gradient is no dense memory (an expanded or strided view): make it contiguous")
+    ptrs = array.array("Q", [g.data_ptr() for g in grads])
+    numel = array.array("q", [g.numel() for g in grads])
+    return ptrs, numel, codes, dev
+
+
+def _is_dense(t):
+    """Whether a tensor's elements are one gapless span of memory, in any order of its dims."""
+    need = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != need:
+            return t.numel() == 0
+        need *= n
+    return True
+
+
+_GRAD_CODES = {torch.float32: F32, torch.bfloat16: BF16}
+
+
+def _grad_norm(grads, norm_type, max_norm, clip, out=None):
+    if norm_type not in NORM_TYPES:
+        raise ValueError(f"norm_type must be 2, inf or 1, got {norm_type}")
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must be a number >= 0, got {max_norm}")
+    ptrs, numel, codes, dev = _grad_arrays(grads)
+    _gpu(grads[0])
+    lib = load_library()
+    n = len(grads)
+    at = numel.buffer_info()[0]
+    if out is None:
+        out = torch.empty(2, dtype=torch.float32, device=dev)
+    wsb = 0 if clip == 2 else lib.ldm_grad_norm_workspace_bytes(at, n)
+    with _on_device(dev):
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+        rc = lib.ldm_grad_norm(ptrs.buffer_info()[0], at, codes, n, NORM_TYPES[norm_type], float(max_norm), clip,
+                               _ptr(out), _ptr(ws), wsb, _stream(out))
+    if rc == ERR_OVERLAP:
+        raise ValueError("gradients overlap in memory (the same gradient twice, or views of one another)")
+    _check(rc, "ldm_grad_norm")
+    return out
+
+
+def grad_norm(grads, norm_type=2.0):
+    """Global norm (2, inf or 1) of a list of dense fp32 / bf16 gradients on one GPU, any mix of types and
+    sizes -> 0-d fp32 device tensor; fp64 sums, no host synchronisation."""
+    return _grad_norm(grads, norm_type, 0.0, 0)[0]
+
+
+def clip_grads(grads, max_norm, norm_type=2.0):
+    """grad_norm, then every gradient times min(1, max_norm / (norm + 1e-6)) in place (nothing is written
+    where the factor is 1) -> the norm before clipping.  Gradients must not overlap."""
+    return _grad_norm(grads, norm_type, max_norm, 1)[0]
