@@ -67,6 +67,26 @@ struct Soft {
     t = fmaf(d, e, t);
     m = hi;
   }
+  // N logits at once, no NaN heeded: one move of the maximum.  It is carried through them: what each passes on is
+  // the lesser of the two, so the set {m, f} becomes {new m} and the f that are left to sum.
+  template <int N> __device__ __forceinline__ void add_all(float (&f)[N], float c2) {
+    float hi = m;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const float v = f[u];
+      f[u] = fminf(hi, v);
+      hi = fmaxf(hi, v);
+    }
+    const float to = hi == -INFINITY ? 0.f : hi;
+    rescale(to, c2);
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const float d = fmaxf(f[u] - to, LOWEST), e = exp2_fast(d * c2);
+      r += e;
+      t = fmaf(d, e, t);
+    }
+    m = hi;
+  }
   __device__ __forceinline__ void join(const Soft& o, float c2) { // o's classes and these
     const float hi = fmaxf(m, o.m), lo = fminf(m, o.m), to = hi == -INFINITY ? 0.f : hi;
     Soft b = o;
@@ -228,33 +248,120 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a) {
   }
 }
 
-// one thread per position
-template <typename T, int K>
-__global__ __launch_bounds__(256) void probs_positions(const Args a) {
-  const int64_t pos = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (pos >= a.positions) return;
-  const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
-  const uint8_t* mask = a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
-  const int64_t y = a.labels ? a.labels[pos] : -1;
-  Soft s;
-  s.clear();
-  Top<K> top;
-  top.clear();
-  bool nan = false;
-  float xy = -INFINITY;
-  for (int c = 0; c < a.classes; ++c) {
-    float v = to_f(x[c * a.sc]);
-    if (mask && !mask[c]) v = -INFINITY;
-    top.add(order_key(v), c);
-    nan |= v != v;
-    xy = c == y ? v : xy;
-    s.add(v, a.c2);
-  }
-  const Result q = result_of(a, s, nan, y, xy);
-  store_result(a, pos, s, q);
+// N adjacent elements at any address aligned to one element: one wide load or store (the card takes unaligned ones)
+template <typename T, int N> struct Pack { T v[N]; };
+template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+  Pack<T, N> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+template <typename T, int N> __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& r) {
+  __builtin_memcpy(p, &r, sizeof(r));
+}
+
+// A group is VEC adjacent positions of one line (n2 of them); the last one of a line reaches back over its
+// neighbour and only its own positions [skip, VEC) are written.
+struct Group { int64_t line, x0, pos; int skip; };
+template <int VEC> __device__ __forceinline__ Group group_of(int64_t g, int64_t per_line, int64_t n2) {
+  Group r;
+  r.line = g / per_line;
+  const int64_t at = (g - r.line * per_line) * VEC;
+  r.x0 = VEC == 1 ? at : min(at, n2 - VEC);
+  r.skip = (int)(at - r.x0);
+  r.pos = r.line * n2 + r.x0;
+  return r;
+}
+template <int VEC, typename T> __device__ __forceinline__ void store_own(T* p, const Pack<T, VEC>& r, int skip) {
+  if (VEC == 1 || skip == 0) {
+    store_pack<T, VEC>(p, r);
+  } else {
 #pragma unroll
-  for (int j = 0; j < K; ++j)
-    if (j < a.k) store_top(a, pos, j, top.key[j], top.id[j], s, q.ls);
+    for (int j = 1; j < VEC; ++j)
+      if (j >= skip) p[j] = r.v[j];
+  }
+}
+
+// Forward over strided classes: a thread has VEC positions of a line, UNR classes of them in registers at a time
+// (their loads are in flight together and the maximum's move costs one rescale).  With SPLIT the block's four waves
+// have the same 64 groups and a quarter of the classes each, joined through LDS: few positions still fill the card.
+template <typename T, int VEC, int K, bool SPLIT>
+__global__ __launch_bounds__(256) void probs_planes(const Args a, int64_t per_line, int64_t groups) {
+  constexpr int UNR = 8;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t want = SPLIT ? (int64_t)blockIdx.x * 64 + lane : (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const bool live = want < groups;
+  if (!SPLIT && !live) return;
+  const Group gr = group_of<VEC>(live ? want : groups - 1, per_line, a.n2);
+  const int64_t i0 = gr.line / a.n1, i1 = gr.line - i0 * a.n1;
+  const T* x = (const T*)a.x + i0 * a.s0 + i1 * a.s1 + gr.x0 * a.s2;
+  const uint8_t* mask = a.mask ? a.mask + (gr.pos / a.mask_div) * a.mask_stride : nullptr;
+  const int c0 = SPLIT ? (int)((int64_t)a.classes * wave >> 2) : 0;
+  const int c1 = SPLIT ? (int)((int64_t)a.classes * (wave + 1) >> 2) : a.classes;
+  int64_t y[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) y[j] = a.labels ? a.labels[gr.pos + j] : -1;
+  Soft s[VEC];
+  Top<K> top[VEC];
+  float xy[VEC];
+  bool nan[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) { s[j].clear(); top[j].clear(); xy[j] = -INFINITY; nan[j] = false; }
+  for (int c = c0; c < c1; c += UNR) {
+    Pack<T, VEC> v[UNR];
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + min(c + u, c1 - 1) * a.sc);
+    bool in[UNR];
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) in[u] = c + u < c1;
+    if (mask)
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) in[u] = in[u] && mask[min(c + u, c1 - 1)];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      float f[UNR];
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) {
+        f[u] = in[u] ? to_f(v[u].v[j]) : -INFINITY;
+        if constexpr (K > 0) top[j].add(order_key(f[u]), c + u);
+        xy[j] = c + u == y[j] ? f[u] : xy[j];
+        nan[j] |= f[u] != f[u];
+      }
+      s[j].template add_all<UNR>(f, a.c2);
+    }
+  }
+  if constexpr (SPLIT) {
+    __shared__ Soft part[4][64 * VEC];
+    __shared__ float part_xy[4][64 * VEC];
+    __shared__ bool part_nan[4][64 * VEC];
+    __shared__ Top<K> part_top[K > 0 ? 4 : 1][K > 0 ? 64 * VEC : 1];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      part[wave][j * 64 + lane] = s[j];
+      part_xy[wave][j * 64 + lane] = xy[j];
+      part_nan[wave][j * 64 + lane] = nan[j];
+      if constexpr (K > 0) part_top[wave][j * 64 + lane] = top[j];
+    }
+    __syncthreads();
+    if (wave || !live) return;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      for (int w = 1; w < 4; ++w) {
+        s[j].join(part[w][j * 64 + lane], a.c2);
+        xy[j] = fmaxf(xy[j], part_xy[w][j * 64 + lane]);   // -inf in all waves but the label's
+        nan[j] |= part_nan[w][j * 64 + lane];
+        if constexpr (K > 0)
+          for (int i = 0; i < K; ++i) top[j].add(part_top[w][j * 64 + lane].key[i], part_top[w][j * 64 + lane].id[i]);
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    if (j < gr.skip) continue;
+    const Result q = result_of(a, s[j], nan[j], y[j], xy[j]);
+    store_result(a, gr.pos + j, s[j], q);
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+      if (i < a.k) store_top(a, gr.pos + j, i, top[j].key[i], top[j].id[i], s[j], q.ls);
+  }
 }
 
 template <typename T>
@@ -292,22 +399,108 @@ __device__ __forceinline__ float grad_of(const BwdArgs<T>& a, const RowGrad& g, 
   return (c == g.label ? g.gl : 0.f) - p * w;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void probs_bwd(const BwdArgs<T> a) {
-  const int64_t pos = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (pos >= a.positions) return;
+// Backward over strided classes: a thread has VEC positions of a line and `span` classes, so that a wave reads
+// and writes whole stretches of a class plane.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, int64_t per_line, int64_t groups,
+                                                        int span) {
+  const int64_t gi = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (gi >= groups) return;
+  const Group gr = group_of<VEC>(gi, per_line, a.n2);
+  const int64_t i0 = gr.line / a.n1, i1 = gr.line - i0 * a.n1;
+  const T* x = a.x + i0 * a.s0 + i1 * a.s1 + gr.x0 * a.s2;
+  T* dx = a.dx + i0 * a.o0 + i1 * a.o1 + gr.x0 * a.o2;
+  const uint8_t* mask = a.mask ? a.mask + (gr.pos / a.mask_div) * a.mask_stride : nullptr;
+  RowGrad g[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) g[j] = row_grad(a, gr.pos + j);
+  const int c0 = blockIdx.y * span, c1 = min(a.classes, c0 + span);
+#pragma unroll 4
+  for (int c = c0; c < c1; ++c) {
+    const Pack<T, VEC> v = load_pack<T, VEC>(x + c * a.sc);
+    const bool out = mask && !mask[c];
+    Pack<T, VEC> d;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) d.v[j] = from_f<T>(out ? 0.f : grad_of(a, g[j], to_f(v.v[j]), c));
+    store_own<VEC, T>(dx + c * a.oc, d, gr.skip);
+  }
+}
+
+// Backward over adjacent classes: a thread has UN packs of VEC classes of one row; a row's last pack reaches back
+// over its neighbour and only its own classes are written.  FLAT: packs of short rows side by side in a block.
+template <typename T, int VEC, int UN, bool FLAT>
+__global__ __launch_bounds__(256) void probs_bwd_rows(const BwdArgs<T> a, unsigned per_row, unsigned blocks_per_row) {
+  int64_t pos;
+  unsigned first;
+  if (FLAT) {
+    const uint64_t q = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    pos = q >> 32 ? (int64_t)(q / per_row) : (int64_t)((uint32_t)q / per_row);
+    first = (unsigned)(q - (uint64_t)pos * per_row);
+    if (pos >= a.positions) return;
+  } else {
+    pos = blockIdx.x / blocks_per_row;
+    first = (blockIdx.x - (unsigned)pos * blocks_per_row) * (256 * UN) + threadIdx.x;
+  }
   const T* x = a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
   T* dx = a.dx + offset_of(pos, a.n1, a.n2, a.o0, a.o1, a.o2);
   const uint8_t* mask = a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
+  Pack<T, VEC> v[UN];
+#pragma unroll
+  for (int u = 0; u < UN; ++u) {
+    const unsigned q = min(first + u * 256, per_row - 1);
+    v[u] = load_pack<T, VEC>(x + min((int)q * VEC, a.classes - VEC));
+  }
   const RowGrad g = row_grad(a, pos);
-  for (int c = 0; c < a.classes; ++c)
-    dx[c * a.oc] = from_f<T>(mask && !mask[c] ? 0.f : grad_of(a, g, to_f(x[c * a.sc]), c));
+#pragma unroll
+  for (int u = 0; u < UN; ++u) {
+    const unsigned q = first + u * 256;
+    if (!FLAT && q >= per_row) break;
+    const int at = (int)q * VEC, c0 = min(at, a.classes - VEC);
+    Pack<T, VEC> d;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) d.v[j] = from_f<T>(grad_of(a, g, to_f(v[u].v[j]), c0 + j));
+    if (mask) {
+      const Pack<uint8_t, VEC> m = load_pack<uint8_t, VEC>(mask + c0);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) d.v[j] = m.v[j] ? d.v[j] : from_f<T>(0.f);
+    }
+    store_own<VEC, T>(dx + c0, d, at - c0);
+  }
 }
 
 bool bad_positions(int64_t n0, int64_t n1, int64_t n2, int64_t classes, int64_t* n) {
   if (n0 < 0 || n1 < 0 || n2 < 0 || classes <= 0 || classes > (1 << 30)) return true;
   *n = n0 * n1 * n2;
   return *n > (1LL << 38);                      // grids stay below 2^31 blocks of 256
+}
+
+template <typename T, int VEC, int K>
+void launch_planes_as(const Args& a, hipStream_t s) {
+  const int64_t per_line = (a.n2 + VEC - 1) / VEC, groups = a.positions / a.n2 * per_line;
+  // four waves to a group where whole groups would leave the card with less than 8 waves a CU
+  if (groups < 64 * 2048 && a.classes >= 16)
+    hipLaunchKernelGGL((probs_planes<T, VEC, K, true>), dim3((unsigned)((groups + 63) / 64)), dim3(256), 0, s, a,
+                       per_line, groups);
+  else
+    hipLaunchKernelGGL((probs_planes<T, VEC, K, false>), dim3((unsigned)((groups + 255) / 256)), dim3(256), 0, s, a,
+                       per_line, groups);
+}
+template <typename T, int VEC>
+void launch_planes_top(const Args& a, hipStream_t s) {
+  if (a.k == 0) launch_planes_as<T, VEC, 0>(a, s);
+  else if (a.k == 1) launch_planes_as<T, VEC, 1>(a, s);
+  else if (a.k == 2) launch_planes_as<T, VEC, 2>(a, s);
+  else if (a.k <= 4) launch_planes_as<T, VEC, 4>(a, s);
+  else if (a.k <= 8) launch_planes_as<T, (VEC > 2 ? 2 : VEC), 8>(a, s);
+  else launch_planes_as<T, 1, 16>(a, s);
+}
+template <typename T>
+int launch_planes(const Args& a, hipStream_t s) {
+  const bool lines = a.s2 == 1 && !(a.mask && a.mask_div % a.n2);
+  if (lines && a.n2 >= 4 && a.positions >= 4 * 64 * 512) launch_planes_top<T, 4>(a, s);
+  else launch_planes_top<T, 1>(a, s);
+  LDM_CHECK_LAUNCH();
+  return LDM_OK;
 }
 
 template <typename T>
@@ -322,12 +515,7 @@ int launch(const Args& a, hipStream_t s) {
     LDM_CHECK_LAUNCH();
     return LDM_OK;
   }
-  const dim3 grid((unsigned)((a.positions + 255) / 256));
-  if (a.k == 0) hipLaunchKernelGGL((probs_positions<T, 0>), grid, block, 0, s, a);
-  else if (a.k <= 4) hipLaunchKernelGGL((probs_positions<T, 4>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((probs_positions<T, 16>), grid, block, 0, s, a);
-  LDM_CHECK_LAUNCH();
-  return LDM_OK;
+  return launch_planes<T>(a, s);
 }
 
 template <typename T>
@@ -341,7 +529,30 @@ int launch_bwd(const ldm_label_probs_bwd_params* p, int64_t n, hipStream_t s) {
   a.mask = (const uint8_t*)p->class_mask; a.mask_stride = p->mask_stride; a.mask_div = p->mask_div;
   a.inv_t = 1.f / p->temperature; a.c2 = (float)(1.4426950408889634 / p->temperature);
   a.stats = p->stats; a.gl = p->d_log_prob; a.ge = p->d_entropy;
-  hipLaunchKernelGGL((probs_bwd<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+  constexpr int RV = 16 / (int)sizeof(T);
+  if (p->sc == 1 && p->oc == 1 && a.classes >= RV) {
+    const unsigned per_row = (unsigned)((a.classes + RV - 1) / RV);
+    if (per_row < 256) {
+      const int64_t blocks = (n * per_row + 255) / 256;
+      if (blocks > 0x7fffffff) return LDM_ERR_ARG;
+      hipLaunchKernelGGL((probs_bwd_rows<T, RV, 1, true>), dim3((unsigned)blocks), dim3(256), 0, s, a, per_row, 1u);
+    } else {
+      const unsigned bpr = (per_row + 511) / 512;
+      if (n * bpr > 0x7fffffff) return LDM_ERR_ARG;
+      hipLaunchKernelGGL((probs_bwd_rows<T, RV, 2, false>), dim3((unsigned)(n * bpr)), dim3(256), 0, s, a, per_row, bpr);
+    }
+    LDM_CHECK_LAUNCH();
+    return LDM_OK;
+  }
+  const bool wide = p->s2 == 1 && p->o2 == 1 && p->n2 >= 4 && !(a.mask && a.mask_div % p->n2);
+  const int vec = wide ? 4 : 1;
+  const int64_t per_line = (p->n2 + vec - 1) / vec, groups = n / p->n2 * per_line, blocks = (groups + 255) / 256;
+  int span = a.classes;                          // 8 classes at least to a thread, 2048 blocks where there is work
+  while (span > 8 && blocks * ((a.classes + span - 1) / span) < 2048) span = (span + 1) / 2;
+  span = std::max(span, (a.classes + 65534) / 65535);
+  const dim3 grid((unsigned)blocks, (unsigned)((a.classes + span - 1) / span));
+  if (wide) hipLaunchKernelGGL((probs_bwd_planes<T, 4>), grid, dim3(256), 0, s, a, per_line, groups, span);
+  else hipLaunchKernelGGL((probs_bwd_planes<T, 1>), grid, dim3(256), 0, s, a, per_line, groups, span);
   LDM_CHECK_LAUNCH();
   return LDM_OK;
 }
