@@ -198,56 +198,6 @@ __device__ __forceinline__ void wave_top(Top<K>& top, int n, int& key, int& id) 
   }
 }
 
-// one block per row of adjacent classes
-template <typename T, int K>
-__global__ __launch_bounds__(256) void probs_rows(const Args a) {
-  __shared__ Soft part[4];
-  __shared__ int part_key[64], part_id[64], part_nan[4];
-  const int64_t pos = blockIdx.x;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
-  const uint8_t* mask = a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
-  Soft s;
-  s.clear();
-  Top<K> top;
-  top.clear();
-  bool nan = false;
-  for (int c = tid; c < a.classes; c += 256) {
-    float v = to_f(x[c]);
-    if (mask && !mask[c]) v = -INFINITY;
-    top.add(order_key(v), c);
-    nan |= v != v;
-    s.add(v, a.c2);
-  }
-  s = wave_join(s, a.c2);
-  if constexpr (K > 0) {
-    int key, id;
-    wave_top<K>(top, a.k, key, id);
-    if (lane < a.k) { part_key[wave * a.k + lane] = key; part_id[wave * a.k + lane] = id; }
-  }
-  if (lane == 0) part[wave] = s;
-  const bool any = __ballot(nan) != 0;
-  if (lane == 0) part_nan[wave] = any;
-  __syncthreads();
-  if (wave) return;
-  s = part[0];
-  for (int w = 1; w < 4; ++w) s.join(part[w], a.c2);
-  nan = part_nan[0] | part_nan[1] | part_nan[2] | part_nan[3];
-  const int64_t y = a.labels ? a.labels[pos] : -1;
-  float xy = -INFINITY;
-  if (y >= 0 && y < a.classes && !(mask && !mask[y])) xy = to_f(x[y]);
-  const Result q = result_of(a, s, nan, y, xy);
-  if (lane == 0) store_result(a, pos, s, q);
-  if constexpr (K > 0) {
-    Top<1> one;
-    one.key[0] = lane < 4 * a.k ? part_key[lane] : KEY_NONE;
-    one.id[0] = lane < 4 * a.k ? part_id[lane] : -1;
-    int key, id;
-    wave_top<1>(one, a.k, key, id);
-    if (lane < a.k) store_top(a, pos, lane, key, id, s, q.ls);
-  }
-}
-
 // N adjacent elements at any address aligned to one element: one wide load or store (the card takes unaligned ones)
 template <typename T, int N> struct Pack { T v[N]; };
 template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
@@ -279,6 +229,239 @@ template <int VEC, typename T> __device__ __forceinline__ void store_own(T* p, c
     for (int j = 1; j < VEC; ++j)
       if (j >= skip) p[j] = r.v[j];
   }
+}
+
+// Short rows of adjacent classes: G lanes to a row, E packs of VEC classes to a lane, all of it in registers.  A
+// row's last pack reaches back over its neighbour; the classes it has in common with it count once.
+template <int G> __device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+template <int G> __device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+template <typename T, int VEC, int G, int E, bool TOP>
+__global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
+  constexpr int N = VEC * E;
+  const int lane = threadIdx.x & 63, sub = lane & (G - 1);
+  const int64_t want = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const bool live = want < a.positions;
+  const int64_t pos = live ? want : a.positions - 1;
+  const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
+  const uint8_t* mask = a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
+  Pack<T, VEC> v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = load_pack<T, VEC>(x + min((sub + e * G) * VEC, a.classes - VEC));
+  const int64_t y = a.labels ? a.labels[pos] : -1;
+  float xy = -INFINITY;
+  if (y >= 0 && y < a.classes && !(mask && !mask[y])) xy = to_f(x[y]);
+  float f[N];
+  int key[TOP ? N : 1];
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int at = (sub + e * G) * VEC, c0 = min(at, a.classes - VEC);
+    Pack<uint8_t, VEC> m;
+    if (mask) m = load_pack<uint8_t, VEC>(mask + c0);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int i = e * VEC + j;
+      const bool in = c0 + j >= at && (!mask || m.v[j]);
+      f[i] = in ? to_f(v[e].v[j]) : -INFINITY;
+      nan |= f[i] != f[i];
+      if constexpr (TOP) key[i] = order_key(f[i]);
+    }
+  }
+  // the lane's maximum is carried out of f; the row's first lane that holds the row's keeps it out of the sums
+  float hi = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float w = f[i];
+    f[i] = fminf(hi, w);
+    hi = fmaxf(hi, w);
+  }
+  Soft s;
+  s.m = lanes_max<G>(hi);
+  const float to = s.m == -INFINITY ? 0.f : s.m;
+  const uint64_t mine = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1)) << (lane & ~(G - 1));
+  const uint64_t holds = __ballot(hi == s.m) & mine;
+  const bool keeper = lane == __ffsll((unsigned long long)holds) - 1;
+  nan = (__ballot(nan) & mine) != 0;
+  const float dh = fmaxf(hi - to, LOWEST), eh = keeper ? 0.f : exp2_fast(dh * a.c2);
+  float r = eh, t = dh * eh;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = fmaxf(f[i] - to, LOWEST), e = exp2_fast(d * a.c2);
+    r += e;
+    t = fmaf(d, e, t);
+  }
+  s.r = lanes_sum<G>(r);
+  s.t = lanes_sum<G>(t);
+  const Result q = result_of(a, s, nan, y, xy);
+  if (live && sub == 0) store_result(a, pos, s, q);
+  if constexpr (TOP) {
+    for (int n = 0; n < a.k; ++n) {
+      int k = KEY_NONE, c = -1;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int ci = min((sub + i / VEC * G) * VEC, a.classes - VEC) + i % VEC;
+        if (key[i] > k) { k = key[i]; c = ci; }
+      }
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) {
+        const int k2 = __shfl_xor(k, o, 64), c2 = __shfl_xor(c, o, 64);
+        if (before(k2, c2, k, c)) { k = k2; c = c2; }
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int ci = min((sub + i / VEC * G) * VEC, a.classes - VEC) + i % VEC;
+        if (ci == c) key[i] = KEY_NONE;
+      }
+      if (live && sub == (n & (G - 1))) store_top(a, pos, n, k, c, s, q.ls);
+    }
+  }
+}
+
+// Long rows of adjacent classes: a block has one segment of one row, its threads packs of VEC classes, UNR of them
+// in flight.  One segment to a row: the block finishes it.  More: what the segments come to goes to the workspace
+// and probs_join finishes the row.
+struct Part { float m, r, t; int nan; };
+template <int K>
+struct RowParts {
+  Soft part[4];
+  int nan[4], key[K > 0 ? 64 : 1], id[K > 0 ? 64 : 1];
+};
+// the block's threads' sums and lists joined, in wave 0 (lane j < k: the j-th of the list); other waves get nothing
+template <int K>
+__device__ __forceinline__ bool block_join_row(RowParts<K>& sh, Soft& s, Top<K>& top, bool& nan, int k, float c2,
+                                               int& key, int& id) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  s = wave_join(s, c2);
+  if constexpr (K > 0) {
+    wave_top<K>(top, k, key, id);
+    if (lane < k) { sh.key[wave * k + lane] = key; sh.id[wave * k + lane] = id; }
+  }
+  const bool any = __ballot(nan) != 0;
+  if (lane == 0) { sh.part[wave] = s; sh.nan[wave] = any; }
+  __syncthreads();
+  if (wave) return false;
+  s = sh.part[0];
+  for (int w = 1; w < 4; ++w) s.join(sh.part[w], c2);
+  nan = sh.nan[0] | sh.nan[1] | sh.nan[2] | sh.nan[3];
+  if constexpr (K > 0) {
+    Top<1> one;
+    one.key[0] = lane < 4 * k ? sh.key[lane] : KEY_NONE;
+    one.id[0] = lane < 4 * k ? sh.id[lane] : -1;
+    wave_top<1>(one, k, key, id);
+  }
+  return true;
+}
+template <typename T>
+__device__ __forceinline__ void finish_row(const Args& a, int64_t pos, const Soft& s, bool nan, int key, int id) {
+  const int lane = threadIdx.x & 63;
+  const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
+  const int64_t y = a.labels ? a.labels[pos] : -1;
+  float xy = -INFINITY;
+  if (y >= 0 && y < a.classes && !(a.mask && !a.mask[(pos / a.mask_div) * a.mask_stride + y])) xy = to_f(x[y]);
+  const Result q = result_of(a, s, nan, y, xy);
+  if (lane == 0) store_result(a, pos, s, q);
+  if (lane < a.k) store_top(a, pos, lane, key, id, s, q.ls);
+}
+
+template <typename T, int VEC, int K>
+__global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, int seg_len, Part* __restrict__ parts,
+                                                  int2* __restrict__ part_top) {
+  constexpr int UNR = 2, N = VEC * UNR;
+  __shared__ RowParts<K> sh;
+  const int64_t pos = segments == 1 ? blockIdx.x : blockIdx.x / segments;
+  const int seg = segments == 1 ? 0 : (int)(blockIdx.x - pos * segments);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
+  const uint8_t* mask = a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
+  const int end = min(a.classes, (seg + 1) * seg_len), last = a.classes - VEC;
+  Soft s;
+  s.clear();
+  Top<K> top;
+  top.clear();
+  bool nan = false;
+  int bar = KEY_NONE;              // the wave's lists hold K keys that are no less
+  for (int base = seg * seg_len; base < end; base += 256 * N) {   // the same turns in every lane: they shuffle
+    const int at0 = base + tid * VEC;
+    Pack<T, VEC> v[UNR];
+    float f[N];
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + min(at0 + u * 256 * VEC, last));
+    bool odd = false;
+    float most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) {
+      const int at = at0 + u * 256 * VEC, c0 = min(at, last);
+      Pack<uint8_t, VEC> m;
+      if (mask) m = load_pack<uint8_t, VEC>(mask + c0);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int i = u * VEC + j;
+        // only the row's last segment ends inside a block's reach, and its last pack reaches back over its neighbour
+        const bool in = at < end && c0 + j >= at && (!mask || m.v[j]);
+        f[i] = in ? to_f(v[u].v[j]) : -INFINITY;
+        odd |= f[i] != f[i];
+        most = fmaxf(most, f[i]);
+      }
+    }
+    nan |= odd;
+    if constexpr (K > 0) {
+      // a class enters only above the K-th key of some lane: later classes lose ties
+      if (__any(odd || order_key(most) > bar)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int k = order_key(f[i]);
+          if (k > bar) top.add(k, min(at0 + i / VEC * 256 * VEC, last) + i % VEC);
+        }
+        bar = top.key[K - 1];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) bar = max(bar, __shfl_xor(bar, o, 64));
+      }
+    }
+    s.template add_all<N>(f, a.c2);
+  }
+  int key = KEY_NONE, id = -1;
+  if (!block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) return;
+  if (segments == 1) {
+    finish_row<T>(a, pos, s, nan, key, id);
+    return;
+  }
+  if (lane == 0) parts[blockIdx.x] = {s.m, s.r, s.t, nan};
+  if (lane < a.k) part_top[(int64_t)blockIdx.x * a.k + lane] = make_int2(key, id);
+}
+
+// one block per row: its segments in the order of their classes
+template <typename T, int K>
+__global__ __launch_bounds__(256) void probs_join(const Args a, int segments, const Part* __restrict__ parts,
+                                                  const int2* __restrict__ part_top) {
+  __shared__ RowParts<K> sh;
+  const int64_t pos = blockIdx.x;
+  Soft s;
+  s.clear();
+  Top<K> top;
+  top.clear();
+  bool nan = false;
+  for (int i = threadIdx.x; i < segments; i += 256) {
+    const Part p = parts[pos * segments + i];
+    Soft o;
+    o.m = p.m; o.r = p.r; o.t = p.t;
+    s.join(o, a.c2);
+    nan |= p.nan != 0;
+    if constexpr (K > 0)
+      for (int j = 0; j < a.k; ++j) {
+        const int2 kc = part_top[(pos * segments + i) * a.k + j];
+        if (kc.y >= 0) top.add(kc.x, kc.y);
+      }
+  }
+  int key = KEY_NONE, id = -1;
+  if (block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) finish_row<T>(a, pos, s, nan, key, id);
 }
 
 // Forward over strided classes: a thread has VEC positions of a line, UNR classes of them in registers at a time
@@ -503,19 +686,60 @@ int launch_planes(const Args& a, hipStream_t s) {
   return LDM_OK;
 }
 
+constexpr int SHORT_CLASSES = 1024;      // at most 16 classes in a lane's registers
+// segments of a long row: whole multiples of a block's reach, 512 blocks at least where rows are few
+int segments_of(int64_t positions, int64_t classes, int dtype) {
+  const int64_t reach = 256 * 16 / (dtype == LDM_BF16 ? 2 : 4);
+  const int64_t most = (classes + reach - 1) / reach;
+  return (int)std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(1, positions)));
+}
+bool long_rows(const ldm_label_probs_params* p) { return p->sc == 1 && p->classes > SHORT_CLASSES; }
+
+template <typename T, int G>
+void launch_short(const Args& a, hipStream_t s) {
+  constexpr int VEC = 16 / (int)sizeof(T), E = 16 / VEC;
+  const dim3 grid((unsigned)((a.positions + 256 / G - 1) / (256 / G)));
+  if (a.k) hipLaunchKernelGGL((probs_short_rows<T, VEC, G, E, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((probs_short_rows<T, VEC, G, E, false>), grid, dim3(256), 0, s, a);
+}
+template <typename T, int K>
+void launch_long_as(const Args& a, int segments, void* ws, hipStream_t s) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int reach = 256 * VEC, per = ((a.classes + reach - 1) / reach + segments - 1) / segments;
+  Part* parts = (Part*)ws;
+  int2* tops = (int2*)(parts + a.positions * segments);
+  hipLaunchKernelGGL((probs_rows<T, VEC, K>), dim3((unsigned)(a.positions * segments)), dim3(256), 0, s, a, segments,
+                     per * reach, parts, tops);
+  if (segments > 1)
+    hipLaunchKernelGGL((probs_join<T, K>), dim3((unsigned)a.positions), dim3(256), 0, s, a, segments, parts, tops);
+}
+
 template <typename T>
-int launch(const Args& a, hipStream_t s) {
-  const dim3 block(256);
-  if (a.sc == 1 && a.classes >= 256) {
-    if (a.positions > 0x7fffffff) return LDM_ERR_ARG;
-    const dim3 grid((unsigned)a.positions);
-    if (a.k == 0) hipLaunchKernelGGL((probs_rows<T, 0>), grid, block, 0, s, a);
-    else if (a.k <= 4) hipLaunchKernelGGL((probs_rows<T, 4>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((probs_rows<T, 16>), grid, block, 0, s, a);
-    LDM_CHECK_LAUNCH();
-    return LDM_OK;
+int launch(const Args& a, void* ws, hipStream_t s) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  if (a.sc == 1 && a.classes > SHORT_CLASSES) {
+    const int segments = segments_of(a.positions, a.classes, sizeof(T) == 2 ? LDM_BF16 : LDM_F32);
+    if (a.positions * segments > 0x7fffffff) return LDM_ERR_ARG;
+    if (a.k == 0) launch_long_as<T, 0>(a, segments, ws, s);
+    else if (a.k == 1) launch_long_as<T, 1>(a, segments, ws, s);
+    else if (a.k <= 4) launch_long_as<T, 4>(a, segments, ws, s);
+    else if (a.k <= 8) launch_long_as<T, 8>(a, segments, ws, s);
+    else launch_long_as<T, 16>(a, segments, ws, s);
+  } else if (a.sc == 1 && a.classes >= VEC) {
+    if (a.positions > (1LL << 32)) return LDM_ERR_ARG;
+    const int lanes = (a.classes + 15) / 16;
+    if (lanes <= 1) launch_short<T, 1>(a, s);
+    else if (lanes <= 2) launch_short<T, 2>(a, s);
+    else if (lanes <= 4) launch_short<T, 4>(a, s);
+    else if (lanes <= 8) launch_short<T, 8>(a, s);
+    else if (lanes <= 16) launch_short<T, 16>(a, s);
+    else if (lanes <= 32) launch_short<T, 32>(a, s);
+    else launch_short<T, 64>(a, s);
+  } else {
+    return launch_planes<T>(a, s);
   }
-  return launch_planes<T>(a, s);
+  LDM_CHECK_LAUNCH();
+  return LDM_OK;
 }
 
 template <typename T>
@@ -562,8 +786,10 @@ bool bad_temperature(float t) { return !(t >= 1e-4f && t <= 1e4f); }
 }  // namespace
 
 extern "C" size_t ldm_label_log_probs_workspace_bytes(const ldm_label_probs_params* p) {
-  (void)p;
-  return 0;
+  if (!p || !long_rows(p) || p->n0 <= 0 || p->n1 <= 0 || p->n2 <= 0) return 0;
+  const int64_t n = p->n0 * p->n1 * p->n2;
+  const int segments = segments_of(n, p->classes, p->dtype);
+  return segments == 1 ? 0 : (size_t)(n * segments) * (sizeof(Part) + sizeof(int2) * (size_t)std::max(0, p->topk));
 }
 
 extern "C" int ldm_label_log_probs(const ldm_label_probs_params* p, ldm_stream_t stream) {
@@ -576,7 +802,8 @@ extern "C" int ldm_label_log_probs(const ldm_label_probs_params* p, ldm_stream_t
   if (!p->logits || !p->entropy || (p->labels && !p->log_prob) || (p->topk && (!p->top_ids || !p->top_log_probs)))
     return LDM_ERR_ARG;
   if (p->inner <= 0 || n % p->inner || (p->class_mask && (p->mask_div <= 0 || p->mask_stride < 0))) return LDM_ERR_ARG;
-  if (p->workspace_bytes < (int64_t)ldm_label_log_probs_workspace_bytes(p)) return LDM_ERR_ARG;
+  const int64_t need = (int64_t)ldm_label_log_probs_workspace_bytes(p);
+  if (need && (!p->workspace || p->workspace_bytes < need)) return LDM_ERR_ARG;
   Args a;
   a.x = p->logits;
   a.n1 = p->n1; a.n2 = p->n2; a.s0 = p->s0; a.s1 = p->s1; a.s2 = p->s2; a.sc = p->sc;
@@ -588,7 +815,7 @@ extern "C" int ldm_label_log_probs(const ldm_label_probs_params* p, ldm_stream_t
   a.lp = p->log_prob; a.ent = p->entropy; a.top_lp = p->top_log_probs; a.top_id = p->top_ids; a.stats = p->stats;
   a.k = p->topk;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  return p->dtype == LDM_BF16 ? launch<bf16_t>(a, s) : launch<float>(a, s);
+  return p->dtype == LDM_BF16 ? launch<bf16_t>(a, p->workspace, s) : launch<float>(a, p->workspace, s);
 }
 
 extern "C" int ldm_label_log_probs_bwd(const ldm_label_probs_bwd_params* p, ldm_stream_t stream) {
