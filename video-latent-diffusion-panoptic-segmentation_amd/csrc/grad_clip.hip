@@ -2,21 +2,25 @@
 //
 //   norm   = sqrt(sum g^2), max |g| or sum |g| over every element of every tensor
 //   factor = min(1, max_norm / (norm + 1e-6));  g *= factor   (torch.nn.utils.clip_grad_norm_)
-// The tensors' addresses travel as kernel arguments, up to TABLE of them to a launch: nothing is
+// The spans' addresses travel as kernel arguments, up to TABLE of them to a launch: nothing is
 // copied to the device, nothing is kept between calls, and a captured graph holds its own table.
 // Squares are summed in fp64 (a square of any fp32 value is finite there), per thread, block and
 // partial in a fixed order: the same gradients give the same bits.
 #include "common.h"
 
-#include <algorithm>
 #include <math.h>
+
+#include <algorithm>
 #include <vector>
 
 namespace {
 
-constexpr int TABLE = 224;               // tensors to a launch: 16 B each, below the 4 KB of kernel arguments
-constexpr int CHUNK = 8192;              // elements a block takes at a time
+constexpr int TABLE = 224;               // spans to a launch: 16 B each, below the 4 KB of kernel arguments
+constexpr int PACKS = 8;                 // 16-byte packs of a chunk to a thread, all in flight: 32 KB to a block
 constexpr int MAX_BLOCKS = 2048;
+
+template <typename T> struct Pack { T v[16 / sizeof(T)]; };
+template <typename T> constexpr int chunk_of() { return 256 * PACKS * 16 / (int)sizeof(T); }
 
 struct Entry {
   uint64_t ptr;                          // bit 63: bf16
@@ -55,22 +59,56 @@ template <int NORM> __device__ __forceinline__ double block_join(double v) {
   return norm_join<NORM>(norm_join<NORM>(part[0], part[1]), norm_join<NORM>(part[2], part[3]));
 }
 
+// A thread's packs of a chunk's elements [0, n), at any address aligned to one element: all loads in flight.
+// pack(index, pack) for each whole one, rest(element) for the elements behind the last.
+template <typename T, typename P, typename R>
+__device__ __forceinline__ void each_pack(const T* g, int n, P pack, R rest) {
+  constexpr int V = 16 / (int)sizeof(T);
+  Pack<T> p[PACKS];
+  if (n == chunk_of<T>()) {
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) __builtin_memcpy(&p[i], g + (i * 256 + threadIdx.x) * V, 16);
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) pack(i * 256 + (int)threadIdx.x, p[i]);
+    return;
+  }
+  const int whole = n / V, last = whole * V + (int)threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < PACKS; ++i)
+    if (i * 256 + (int)threadIdx.x < whole) __builtin_memcpy(&p[i], g + (i * 256 + threadIdx.x) * V, 16);
+  if (last < n) rest(last);
+#pragma unroll
+  for (int i = 0; i < PACKS; ++i)
+    if (i * 256 + (int)threadIdx.x < whole) pack(i * 256 + (int)threadIdx.x, p[i]);
+}
+
 template <int NORM, typename T>
-__device__ __forceinline__ double chunk_norm(const T* g, int64_t n, double acc) {
-  for (int64_t i = threadIdx.x; i < n; i += 256) acc = norm_add<NORM>(acc, to_f(g[i]));
+__device__ __forceinline__ double chunk_norm(const T* g, int n, double acc) {
+  each_pack(g, n, [&](int, const Pack<T>& p) {
+#pragma unroll
+    for (int j = 0; j < 16 / (int)sizeof(T); ++j) acc = norm_add<NORM>(acc, to_f(p.v[j]));
+  }, [&](int i) { acc = norm_add<NORM>(acc, to_f(g[i])); });
   return acc;
+}
+
+// chunk c of a table: calls f(pointer, elements) with the span's type
+template <typename F> __device__ __forceinline__ void with_chunk(const Table& t, int c, F f) {
+  const Entry e = t.e[entry_of(t, c)];
+  const int64_t k = c - (int)e.chunk0;
+  if (e.ptr >> 63) {
+    const int64_t at = k * chunk_of<bf16_t>();
+    f((bf16_t*)(e.ptr & ~(1ull << 63)) + at, (int)min((int64_t)chunk_of<bf16_t>(), (int64_t)e.n - at));
+  } else {
+    const int64_t at = k * chunk_of<float>();
+    f((float*)e.ptr + at, (int)min((int64_t)chunk_of<float>(), (int64_t)e.n - at));
+  }
 }
 
 template <int NORM>
 __global__ __launch_bounds__(256) void norm_parts(const Table t, double* __restrict__ part) {
   double acc = 0.0;
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    const Entry e = t.e[entry_of(t, c)];
-    const int64_t at = (int64_t)(c - (int)e.chunk0) * CHUNK;
-    const int64_t n = min((int64_t)CHUNK, (int64_t)e.n - at);
-    if (e.ptr >> 63) acc = chunk_norm<NORM>((const bf16_t*)(e.ptr & ~(1ull << 63)) + at, n, acc);
-    else acc = chunk_norm<NORM>((const float*)e.ptr + at, n, acc);
-  }
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x)
+    with_chunk(t, c, [&](const auto* g, int n) { acc = chunk_norm<NORM>(g, n, acc); });
   acc = block_join<NORM>(acc);
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
 }
@@ -96,25 +134,26 @@ __global__ __launch_bounds__(256) void norm_final(const double* __restrict__ par
 // a gradient is multiplied by the factor as its own type holds it and rounded once, as torch's in-place product
 // of a tensor with a device scalar is: a bf16 gradient's factor has 8 bits
 template <typename T>
-__device__ __forceinline__ void chunk_scale(T* g, int64_t n, float factor) {
+__device__ __forceinline__ void chunk_scale(T* g, int n, float factor) {
+  constexpr int V = 16 / (int)sizeof(T);
   const float f = to_f(from_f<T>(factor));
   if (f == 1.f) return;
-  for (int64_t i = threadIdx.x; i < n; i += 256) g[i] = from_f<T>(to_f(g[i]) * f);
+  each_pack(g, n, [&](int i, Pack<T> p) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) p.v[j] = from_f<T>(to_f(p.v[j]) * f);
+    __builtin_memcpy(g + i * V, &p, 16);
+  }, [&](int i) { g[i] = from_f<T>(to_f(g[i]) * f); });
 }
 
+// the last chunks first: the norm's pass has left them in the memory-side cache
 __global__ __launch_bounds__(256) void scale_all(const Table t, const float* __restrict__ out) {
   const float f = out[1];
   if (f == 1.f) return;
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    const Entry e = t.e[entry_of(t, c)];
-    const int64_t at = (int64_t)(c - (int)e.chunk0) * CHUNK;
-    const int64_t n = min((int64_t)CHUNK, (int64_t)e.n - at);
-    if (e.ptr >> 63) chunk_scale((bf16_t*)(e.ptr & ~(1ull << 63)) + at, n, f);
-    else chunk_scale((float*)e.ptr + at, n, f);
-  }
+  for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x)
+    with_chunk(t, c, [&](auto* g, int n) { chunk_scale(g, n, f); });
 }
 
-// a tensor above 2^30 elements is listed in pieces
+// a span above 2^30 elements is listed in pieces (of whole chunks)
 constexpr int64_t PIECE = 1LL << 30;
 int64_t entries_of(const int64_t* numel, int n) {
   int64_t c = 0;
@@ -141,7 +180,8 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
   if (norm_type < LDM_NORM_2 || norm_type > LDM_NORM_1 || !(max_norm >= 0.0)) return LDM_ERR_ARG;
   const int64_t need = clip == 2 ? 0 : (int64_t)ldm_grad_norm_workspace_bytes(numel, ntensors);
   if (need && (!workspace || workspace_bytes < need)) return LDM_ERR_ARG;
-  struct Span { uint64_t lo, hi; };
+  // Tensors in the order of their addresses; those that lie back to back (views of a bucket) are one span.
+  struct Span { uint64_t lo, hi, size; };
   std::vector<Span> spans;
   std::vector<Table> tables;
   try {
@@ -153,25 +193,34 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
       const uint64_t size = dtypes[i] == LDM_BF16 ? 2 : 4;
       if (!a || (a >> 63)) return LDM_ERR_ARG;
       if (a % size) return LDM_ERR_ALIGN;
-      spans.push_back({a, a + size * (uint64_t)numel[i]});
-      for (int64_t at = 0; at < numel[i]; at += PIECE) {
+      spans.push_back({a, a + size * (uint64_t)numel[i], size});
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span& p, const Span& q) { return p.lo < q.lo; });
+    size_t last = 0;
+    for (size_t i = 1; i < spans.size(); ++i) {
+      if (spans[i].lo < spans[last].hi) return LDM_ERR_OVERLAP;
+      if (spans[i].lo == spans[last].hi && spans[i].size == spans[last].size) spans[last].hi = spans[i].hi;
+      else spans[++last] = spans[i];
+    }
+    if (!spans.empty()) spans.resize(last + 1);
+    for (const Span& p : spans) {
+      const int64_t total = (int64_t)((p.hi - p.lo) / p.size);
+      const int64_t chunk = p.size == 2 ? chunk_of<bf16_t>() : chunk_of<float>();
+      for (int64_t at = 0; at < total; at += PIECE) {
         if (tables.empty() || tables.back().count == TABLE) {
           tables.emplace_back();
           tables.back().count = tables.back().chunks = 0;
         }
         Table& t = tables.back();
-        const int64_t n = std::min(PIECE, numel[i] - at);
-        t.e[t.count++] = {(a + size * (uint64_t)at) | ((uint64_t)(dtypes[i] == LDM_BF16) << 63), (uint32_t)n,
+        const int64_t n = std::min(PIECE, total - at);
+        t.e[t.count++] = {(p.lo + p.size * (uint64_t)at) | ((uint64_t)(p.size == 2) << 63), (uint32_t)n,
                           (uint32_t)t.chunks};
-        t.chunks += (int)((n + CHUNK - 1) / CHUNK);
+        t.chunks += (int)((n + chunk - 1) / chunk);
       }
     }
-    std::sort(spans.begin(), spans.end(), [](const Span& p, const Span& q) { return p.lo < q.lo; });
   } catch (...) {
     return LDM_ERR_ARG;
   }
-  for (size_t i = 1; i < spans.size(); ++i)
-    if (spans[i].lo < spans[i - 1].hi) return LDM_ERR_OVERLAP;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(workspace);
   if (clip != 2) {
@@ -193,7 +242,8 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
     LDM_CHECK_LAUNCH();
   }
   if (clip)
-    for (const Table& t : tables) {
+    for (size_t i = tables.size(); i-- > 0;) {
+      const Table& t = tables[i];
       hipLaunchKernelGGL(scale_all, dim3(std::min(t.chunks, MAX_BLOCKS)), dim3(256), 0, s, t, out);
       LDM_CHECK_LAUNCH();
     }
