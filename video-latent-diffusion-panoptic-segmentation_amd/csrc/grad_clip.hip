@@ -119,16 +119,21 @@ __device__ __forceinline__ float factor_of(float norm, float max_norm) {
   return f > 1.f ? 1.f : f;
 }
 
+// the partials joined: the norm and the factor, in every thread of the block
 template <int NORM>
-__global__ __launch_bounds__(256) void norm_final(const double* __restrict__ part, int parts, float max_norm,
-                                                  float* __restrict__ out) {
+__device__ __forceinline__ float2 norm_of(const double* __restrict__ part, int parts, float max_norm) {
   double acc = 0.0;
   for (int i = threadIdx.x; i < parts; i += 256) acc = norm_join<NORM>(acc, part[i]);
   acc = block_join<NORM>(acc);
-  if (threadIdx.x == 0) {
-    out[0] = (float)(NORM == LDM_NORM_2 ? sqrt(acc) : acc);
-    out[1] = factor_of(out[0], max_norm);
-  }
+  const float norm = (float)(NORM == LDM_NORM_2 ? sqrt(acc) : acc);
+  return make_float2(norm, factor_of(norm, max_norm));
+}
+
+template <int NORM>
+__global__ __launch_bounds__(256) void norm_final(const double* __restrict__ part, int parts, float max_norm,
+                                                  float* __restrict__ out) {
+  const float2 r = norm_of<NORM>(part, parts, max_norm);
+  if (threadIdx.x == 0) { out[0] = r.x; out[1] = r.y; }
 }
 
 // a gradient is multiplied by the factor as its own type holds it and rounded once, as torch's in-place product
@@ -146,11 +151,21 @@ __device__ __forceinline__ void chunk_scale(T* g, int n, float factor) {
 }
 
 // the last chunks first: the norm's pass has left them in the memory-side cache
-__global__ __launch_bounds__(256) void scale_all(const Table t, const float* __restrict__ out) {
-  const float f = out[1];
+__device__ __forceinline__ void scale_chunks(const Table& t, float f) {
   if (f == 1.f) return;
   for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x)
     with_chunk(t, c, [&](auto* g, int n) { chunk_scale(g, n, f); });
+}
+__global__ __launch_bounds__(256) void scale_all(const Table t, const float* __restrict__ out) {
+  scale_chunks(t, out[1]);
+}
+// the same for one table with few partials: every block joins them itself, which takes a launch less
+template <int NORM>
+__global__ __launch_bounds__(256) void scale_joined(const Table t, const double* __restrict__ part, int parts,
+                                                    float max_norm, float* __restrict__ out) {
+  const float2 r = norm_of<NORM>(part, parts, max_norm);
+  if (blockIdx.x == 0 && threadIdx.x == 0) { out[0] = r.x; out[1] = r.y; }
+  scale_chunks(t, r.y);
 }
 
 // a span above 2^30 elements is listed in pieces (of whole chunks)
@@ -161,9 +176,33 @@ int64_t entries_of(const int64_t* numel, int n) {
   return c;
 }
 
+constexpr int JOIN_PARTS = 512;          // two partials a thread
+
 template <int NORM>
-void launch_norm(const Table& t, int blocks, double* part, hipStream_t s) {
-  hipLaunchKernelGGL((norm_parts<NORM>), dim3(blocks), dim3(256), 0, s, t, part);
+int launch(const std::vector<Table>& tables, float max_norm, int clip, float* out, double* part, hipStream_t s) {
+  int parts = 0;
+  if (clip != 2) {
+    for (const Table& t : tables) {
+      const int blocks = std::min(t.chunks, MAX_BLOCKS);
+      hipLaunchKernelGGL((norm_parts<NORM>), dim3(blocks), dim3(256), 0, s, t, part + parts);
+      LDM_CHECK_LAUNCH();
+      parts += blocks;
+    }
+    if (clip == 1 && tables.size() == 1 && parts <= JOIN_PARTS) {
+      hipLaunchKernelGGL((scale_joined<NORM>), dim3(parts), dim3(256), 0, s, tables[0], part, parts, max_norm, out);
+      LDM_CHECK_LAUNCH();
+      return LDM_OK;
+    }
+    hipLaunchKernelGGL((norm_final<NORM>), dim3(1), dim3(256), 0, s, part, parts, max_norm, out);
+    LDM_CHECK_LAUNCH();
+  }
+  if (clip)
+    for (size_t i = tables.size(); i-- > 0;) {
+      const Table& t = tables[i];
+      hipLaunchKernelGGL(scale_all, dim3(std::min(t.chunks, MAX_BLOCKS)), dim3(256), 0, s, t, out);
+      LDM_CHECK_LAUNCH();
+    }
+  return LDM_OK;
 }
 
 }  // namespace
@@ -223,29 +262,7 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
   }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(workspace);
-  if (clip != 2) {
-    int parts = 0;
-    for (const Table& t : tables) {
-      const int blocks = std::min(t.chunks, MAX_BLOCKS);
-      if (norm_type == LDM_NORM_2) launch_norm<LDM_NORM_2>(t, blocks, part + parts, s);
-      else if (norm_type == LDM_NORM_INF) launch_norm<LDM_NORM_INF>(t, blocks, part + parts, s);
-      else launch_norm<LDM_NORM_1>(t, blocks, part + parts, s);
-      LDM_CHECK_LAUNCH();
-      parts += blocks;
-    }
-    if (norm_type == LDM_NORM_2)
-      hipLaunchKernelGGL((norm_final<LDM_NORM_2>), dim3(1), dim3(256), 0, s, part, parts, (float)max_norm, out);
-    else if (norm_type == LDM_NORM_INF)
-      hipLaunchKernelGGL((norm_final<LDM_NORM_INF>), dim3(1), dim3(256), 0, s, part, parts, (float)max_norm, out);
-    else
-      hipLaunchKernelGGL((norm_final<LDM_NORM_1>), dim3(1), dim3(256), 0, s, part, parts, (float)max_norm, out);
-    LDM_CHECK_LAUNCH();
-  }
-  if (clip)
-    for (size_t i = tables.size(); i-- > 0;) {
-      const Table& t = tables[i];
-      hipLaunchKernelGGL(scale_all, dim3(std::min(t.chunks, MAX_BLOCKS)), dim3(256), 0, s, t, out);
-      LDM_CHECK_LAUNCH();
-    }
-  return LDM_OK;
+  if (norm_type == LDM_NORM_2) return launch<LDM_NORM_2>(tables, (float)max_norm, clip, out, part, s);
+  if (norm_type == LDM_NORM_INF) return launch<LDM_NORM_INF>(tables, (float)max_norm, clip, out, part, s);
+  return launch<LDM_NORM_1>(tables, (float)max_norm, clip, out, part, s);
 }
