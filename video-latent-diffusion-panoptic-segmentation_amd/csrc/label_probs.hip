@@ -50,6 +50,19 @@ __device__ __forceinline__ float key_value(int k) {
 }
 constexpr int KEY_NONE = (int)0x807fffff;   // order_key(-inf): a class without probability is no candidate
 
+// v_max / v_min as they are: fmaxf of a loaded value costs one more to quieten signalling NaNs, and a row with any
+// NaN is known by other means
+__device__ __forceinline__ float raw_max(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ float raw_min(float a, float b) {
+  float r;
+  asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+
 // running maximum and sums of one set of logits; the maximum's own term is in neither sum
 struct Soft {
   float m, r, t;
@@ -74,8 +87,8 @@ struct Soft {
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       const float v = f[u];
-      f[u] = fminf(hi, v);
-      hi = fmaxf(hi, v);
+      f[u] = raw_min(hi, v);
+      hi = raw_max(hi, v);
     }
     const float to = hi == -INFINITY ? 0.f : hi;
     rescale(to, c2);
@@ -122,30 +135,26 @@ struct Top {
   }
 };
 
+// log(1 + r), r >= 0, to a few roundings of itself: what 1 + r loses, r / ((1 + r) - 1) gives back (Goldberg 1991)
+__device__ __forceinline__ float log1p_of(float r) {
+  const float w = 1.f + r, l = LN2 * __builtin_amdgcn_logf(w);
+  return w == 1.f ? r : l * (r * __builtin_amdgcn_rcpf(w - 1.f));
+}
+
 // what a position's sums come to
 struct Result { float ls, ent, lp; int label; };
 __device__ __forceinline__ Result result_of(const Args& a, const Soft& s, bool nan, int64_t y, float xy) {
   Result q;
   const float none = __int_as_float(0x7fc00000);
   const bool empty = s.m == -INFINITY, bad = nan || s.m == INFINITY;
-  q.ls = bad ? none : log1pf(s.r);
-  q.ent = bad ? none : empty ? 0.f : q.ls - s.t * a.inv_t / (1.f + s.r);
+  q.ls = bad ? none : log1p_of(s.r);
+  q.ent = bad ? none : empty ? 0.f : q.ls - s.t * a.inv_t * __builtin_amdgcn_rcpf(1.f + s.r);
   const bool known = !(a.has_ignore && y == a.ignore), inside = y >= 0 && y < a.classes;
   if (!known) q.lp = 0.f;
   else if (!inside || bad) q.lp = none;
   else q.lp = xy == -INFINITY ? -INFINITY : (xy - s.m) * a.inv_t - q.ls;
   q.label = known && inside && q.lp > -INFINITY ? (int)y : -1;   // NaN > -inf is false: the row is NaN anyway
   return q;
-}
-__device__ __forceinline__ void store_result(const Args& a, int64_t pos, const Soft& s, const Result& q) {
-  a.ent[pos] = q.ent;
-  if (a.labels) a.lp[pos] = q.lp;
-  if (a.stats) {
-    a.stats[pos] = s.m;
-    a.stats[a.positions + pos] = q.ls;
-    a.stats[2 * a.positions + pos] = q.ent;
-    a.stats[3 * a.positions + pos] = __int_as_float(a.labels ? q.label : -1);
-  }
 }
 __device__ __forceinline__ void store_top(const Args& a, int64_t pos, int j, int key, int id, const Soft& s, float ls) {
   const int64_t o = pos / a.inner, at = (o * a.k + j) * a.inner + (pos - o * a.inner);
@@ -231,6 +240,31 @@ template <int VEC, typename T> __device__ __forceinline__ void store_own(T* p, c
   }
 }
 
+template <int VEC>
+__device__ __forceinline__ void store_results(const Args& a, int64_t pos, int skip, const Soft (&s)[VEC],
+                                              const Result (&q)[VEC]) {
+  Pack<float, VEC> ent, lp, m, ls, y;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    ent.v[j] = q[j].ent; lp.v[j] = q[j].lp; m.v[j] = s[j].m; ls.v[j] = q[j].ls;
+    y.v[j] = __int_as_float(a.labels ? q[j].label : -1);
+  }
+  store_own<VEC>(a.ent + pos, ent, skip);
+  if (a.labels) store_own<VEC>(a.lp + pos, lp, skip);
+  if (a.stats) {
+    store_own<VEC>(a.stats + pos, m, skip);
+    store_own<VEC>(a.stats + a.positions + pos, ls, skip);
+    store_own<VEC>(a.stats + 2 * a.positions + pos, ent, skip);
+    store_own<VEC>(a.stats + 3 * a.positions + pos, y, skip);
+  }
+}
+
+__device__ __forceinline__ void store_row(const Args& a, int64_t pos, const Soft& s, const Result& q) {
+  const Soft one[1] = {s};
+  const Result res[1] = {q};
+  store_results<1>(a, pos, 0, one, res);
+}
+
 // Short rows of adjacent classes: G lanes to a row, E packs of VEC classes to a lane, all of it in registers.  A
 // row's last pack reaches back over its neighbour; the classes it has in common with it count once.
 template <int G> __device__ __forceinline__ float lanes_max(float v) {
@@ -301,7 +335,7 @@ __global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
   s.r = lanes_sum<G>(r);
   s.t = lanes_sum<G>(t);
   const Result q = result_of(a, s, nan, y, xy);
-  if (live && sub == 0) store_result(a, pos, s, q);
+  if (live && sub == 0) store_row(a, pos, s, q);
   if constexpr (TOP) {
     for (int n = 0; n < a.k; ++n) {
       int k = KEY_NONE, c = -1;
@@ -367,7 +401,7 @@ __device__ __forceinline__ void finish_row(const Args& a, int64_t pos, const Sof
   float xy = -INFINITY;
   if (y >= 0 && y < a.classes && !(a.mask && !a.mask[(pos / a.mask_div) * a.mask_stride + y])) xy = to_f(x[y]);
   const Result q = result_of(a, s, nan, y, xy);
-  if (lane == 0) store_result(a, pos, s, q);
+  if (lane == 0) store_row(a, pos, s, q);
   if (lane < a.k) store_top(a, pos, lane, key, id, s, q.ls);
 }
 
@@ -464,6 +498,32 @@ __global__ __launch_bounds__(256) void probs_join(const Args a, int segments, co
   if (block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) finish_row<T>(a, pos, s, nan, key, id);
 }
 
+// What a thread of probs_planes keeps of the most likely classes of one position: values in falling order.  A new
+// value's place is the median of its neighbours (v_med3); a later class needs a larger value.  NaNs are sorted out
+// afterwards (nan_first): here they compare false.
+template <int K>
+struct TopValues {
+  float v[K > 0 ? K : 1];
+  int id[K > 0 ? K : 1];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < K; ++i) { v[i] = -INFINITY; id[i] = -1; }
+  }
+  __device__ __forceinline__ void add(float f, int c) {
+    if constexpr (K > 0) {
+      bool over[K];
+#pragma unroll
+      for (int i = 0; i < K; ++i) over[i] = f > v[i];
+#pragma unroll
+      for (int i = K - 1; i > 0; --i) {
+        v[i] = __builtin_amdgcn_fmed3f(v[i - 1], f, v[i]);
+        id[i] = over[i - 1] ? id[i - 1] : over[i] ? c : id[i];
+      }
+      id[0] = over[0] ? c : id[0];
+      v[0] = over[0] ? f : v[0];
+    }
+  }
+};
 // Forward over strided classes: a thread has VEC positions of a line, UNR classes of them in registers at a time
 // (their loads are in flight together and the maximum's move costs one rescale).  With SPLIT the block's four waves
 // have the same 64 groups and a quarter of the classes each, joined through LDS: few positions still fill the card.
@@ -481,69 +541,143 @@ __global__ __launch_bounds__(256) void probs_planes(const Args a, int64_t per_li
   const int c0 = SPLIT ? (int)((int64_t)a.classes * wave >> 2) : 0;
   const int c1 = SPLIT ? (int)((int64_t)a.classes * (wave + 1) >> 2) : a.classes;
   int64_t y[VEC];
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) y[j] = a.labels ? a.labels[gr.pos + j] : -1;
-  Soft s[VEC];
-  Top<K> top[VEC];
   float xy[VEC];
+  if (!SPLIT || wave == 0) {
+    // the label's logit is fetched beside the loop, which reads its line as well
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      y[j] = a.labels ? a.labels[gr.pos + j] : -1;
+      xy[j] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (y[j] >= 0 && y[j] < a.classes && !(mask && !mask[y[j]])) xy[j] = to_f(x[y[j] * a.sc + j * a.s2]);
+  }
+  Soft s[VEC];
+  TopValues<K> top[VEC];
   bool nan[VEC];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) { s[j].clear(); top[j].clear(); xy[j] = -INFINITY; nan[j] = false; }
-  for (int c = c0; c < c1; c += UNR) {
-    Pack<T, VEC> v[UNR];
+  for (int j = 0; j < VEC; ++j) { s[j].clear(); top[j].clear(); nan[j] = false; }
+  auto chunk = [&](int c, const Pack<float, VEC> (&v)[UNR]) {
+    if constexpr (K > 0) {
 #pragma unroll
-    for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + min(c + u, c1 - 1) * a.sc);
-    bool in[UNR];
+      for (int u = 0; u < UNR; ++u) {
+        bool enter = false;
 #pragma unroll
-    for (int u = 0; u < UNR; ++u) in[u] = c + u < c1;
-    if (mask)
+        for (int j = 0; j < VEC; ++j) enter |= v[u].v[j] > top[j].v[K - 1];
+        if (__any(enter))
 #pragma unroll
-      for (int u = 0; u < UNR; ++u) in[u] = in[u] && mask[min(c + u, c1 - 1)];
+          for (int j = 0; j < VEC; ++j) top[j].add(v[u].v[j], c + u);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       float f[UNR];
 #pragma unroll
       for (int u = 0; u < UNR; ++u) {
-        f[u] = in[u] ? to_f(v[u].v[j]) : -INFINITY;
-        if constexpr (K > 0) top[j].add(order_key(f[u]), c + u);
-        xy[j] = c + u == y[j] ? f[u] : xy[j];
+        f[u] = v[u].v[j];
         nan[j] |= f[u] != f[u];
       }
       s[j].template add_all<UNR>(f, a.c2);
     }
+  };
+  int c = c0;
+  if (!mask)
+    for (; c + UNR <= c1; c += UNR) {
+      Pack<T, VEC> v[UNR];
+      Pack<float, VEC> f[UNR];
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + (c + u) * a.sc);
+#pragma unroll
+      for (int u = 0; u < UNR; ++u)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[u].v[j] = to_f(v[u].v[j]);
+      chunk(c, f);
+    }
+  for (; c < c1; c += UNR) {
+    Pack<T, VEC> v[UNR];
+    Pack<float, VEC> f[UNR];
+    bool in[UNR];
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) {
+      const int cu = min(c + u, c1 - 1);
+      v[u] = load_pack<T, VEC>(x + cu * a.sc);
+      in[u] = c + u < c1 && (!mask || mask[cu]);
+    }
+#pragma unroll
+    for (int u = 0; u < UNR; ++u)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[u].v[j] = in[u] ? to_f(v[u].v[j]) : -INFINITY;
+    chunk(c, f);
   }
   if constexpr (SPLIT) {
     __shared__ Soft part[4][64 * VEC];
-    __shared__ float part_xy[4][64 * VEC];
     __shared__ bool part_nan[4][64 * VEC];
-    __shared__ Top<K> part_top[K > 0 ? 4 : 1][K > 0 ? 64 * VEC : 1];
+    __shared__ TopValues<K> part_top[K > 0 ? 4 : 1][K > 0 ? 64 * VEC : 1];
+    if (wave)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      part[wave][j * 64 + lane] = s[j];
-      part_xy[wave][j * 64 + lane] = xy[j];
-      part_nan[wave][j * 64 + lane] = nan[j];
-      if constexpr (K > 0) part_top[wave][j * 64 + lane] = top[j];
-    }
+      for (int j = 0; j < VEC; ++j) {
+        part[wave][j * 64 + lane] = s[j];
+        part_nan[wave][j * 64 + lane] = nan[j];
+        if constexpr (K > 0) part_top[wave][j * 64 + lane] = top[j];
+      }
     __syncthreads();
     if (wave || !live) return;
 #pragma unroll
     for (int j = 0; j < VEC; ++j)
       for (int w = 1; w < 4; ++w) {
         s[j].join(part[w][j * 64 + lane], a.c2);
-        xy[j] = fmaxf(xy[j], part_xy[w][j * 64 + lane]);   // -inf in all waves but the label's
         nan[j] |= part_nan[w][j * 64 + lane];
         if constexpr (K > 0)
-          for (int i = 0; i < K; ++i) top[j].add(part_top[w][j * 64 + lane].key[i], part_top[w][j * 64 + lane].id[i]);
+#pragma unroll
+          for (int i = 0; i < K; ++i) top[j].add(part_top[w][j * 64 + lane].v[i], part_top[w][j * 64 + lane].id[i]);
       }
   }
+  Result q[VEC];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    if (j < gr.skip) continue;
-    const Result q = result_of(a, s[j], nan[j], y[j], xy[j]);
-    store_result(a, gr.pos + j, s[j], q);
+  for (int j = 0; j < VEC; ++j) q[j] = result_of(a, s[j], nan[j], y[j], xy[j]);
+  store_results<VEC>(a, gr.pos, gr.skip, s, q);
+  if constexpr (K > 0) {
+    // positions behind the class dim: a line lies in one of their runs, or there are none
+    const int64_t o = a.inner == 1 ? gr.pos : gr.pos / a.inner;
 #pragma unroll
     for (int i = 0; i < K; ++i)
-      if (i < a.k) store_top(a, gr.pos + j, i, top[j].key[i], top[j].id[i], s[j], q.ls);
+      if (i < a.k) {
+        Pack<float, VEC> lp;
+        Pack<int, VEC> id;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          id.v[j] = top[j].id[i];
+          lp.v[j] = id.v[j] < 0 ? -INFINITY : (top[j].v[i] - s[j].m) * a.inv_t - q[j].ls;
+        }
+        if (a.inner == 1) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (j >= gr.skip) {
+              a.top_lp[(gr.pos + j) * a.k + i] = lp.v[j];
+              a.top_id[(gr.pos + j) * a.k + i] = id.v[j];
+            }
+        } else {
+          const int64_t at = (o * a.k + i) * a.inner + gr.pos - o * a.inner;
+          store_own<VEC>(a.top_lp + at, lp, gr.skip);
+          store_own<VEC>(a.top_id + at, id, gr.skip);
+        }
+      }
+    // a position that has NaNs (all its values are): those classes first, lower class first, then by value
+    int redo = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) redo |= nan[j] && j >= gr.skip ? 1 << j : 0;
+    for (; redo; redo &= redo - 1) {
+      const int j = __ffs(redo) - 1;
+      Top<K> keys;
+      keys.clear();
+      for (int k = 0; k < a.classes; ++k)
+        if (!mask || mask[k]) keys.add(order_key(to_f(x[k * a.sc + j * a.s2])), k);
+      const int64_t at = o * a.k * a.inner + (a.inner == 1 ? j * a.k : gr.pos - o * a.inner + j);
+#pragma unroll
+      for (int i = 0; i < K; ++i)
+        if (i < a.k) a.top_id[at + i * a.inner] = keys.id[i];
+    }
   }
 }
 
@@ -605,7 +739,7 @@ __global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, int6
     Pack<T, VEC> d;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) d.v[j] = from_f<T>(out ? 0.f : grad_of(a, g[j], to_f(v.v[j]), c));
-    store_own<VEC, T>(dx + c * a.oc, d, gr.skip);
+    store_own<VEC>(dx + c * a.oc, d, gr.skip);
   }
 }
 
@@ -647,7 +781,7 @@ __global__ __launch_bounds__(256) void probs_bwd_rows(const BwdArgs<T> a, unsign
 #pragma unroll
       for (int j = 0; j < VEC; ++j) d.v[j] = m.v[j] ? d.v[j] : from_f<T>(0.f);
     }
-    store_own<VEC, T>(dx + c0, d, at - c0);
+    store_own<VEC>(dx + c0, d, at - c0);
   }
 }
 
