@@ -218,18 +218,6 @@ template <typename T, int N> __device__ __forceinline__ void store_pack(T* p, co
   __builtin_memcpy(p, &r, sizeof(r));
 }
 
-// A group is VEC adjacent positions of one line (n2 of them); the last one of a line reaches back over its
-// neighbour and only its own positions [skip, VEC) are written.
-struct Group { int64_t line, x0, pos; int skip; };
-template <int VEC> __device__ __forceinline__ Group group_of(int64_t g, int64_t per_line, int64_t n2) {
-  Group r;
-  r.line = g / per_line;
-  const int64_t at = (g - r.line * per_line) * VEC;
-  r.x0 = VEC == 1 ? at : min(at, n2 - VEC);
-  r.skip = (int)(at - r.x0);
-  r.pos = r.line * n2 + r.x0;
-  return r;
-}
 template <int VEC, typename T> __device__ __forceinline__ void store_own(T* p, const Pack<T, VEC>& r, int skip) {
   if (VEC == 1 || skip == 0) {
     store_pack<T, VEC>(p, r);
@@ -240,29 +228,15 @@ template <int VEC, typename T> __device__ __forceinline__ void store_own(T* p, c
   }
 }
 
-template <int VEC>
-__device__ __forceinline__ void store_results(const Args& a, int64_t pos, int skip, const Soft (&s)[VEC],
-                                              const Result (&q)[VEC]) {
-  Pack<float, VEC> ent, lp, m, ls, y;
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    ent.v[j] = q[j].ent; lp.v[j] = q[j].lp; m.v[j] = s[j].m; ls.v[j] = q[j].ls;
-    y.v[j] = __int_as_float(a.labels ? q[j].label : -1);
-  }
-  store_own<VEC>(a.ent + pos, ent, skip);
-  if (a.labels) store_own<VEC>(a.lp + pos, lp, skip);
-  if (a.stats) {
-    store_own<VEC>(a.stats + pos, m, skip);
-    store_own<VEC>(a.stats + a.positions + pos, ls, skip);
-    store_own<VEC>(a.stats + 2 * a.positions + pos, ent, skip);
-    store_own<VEC>(a.stats + 3 * a.positions + pos, y, skip);
-  }
-}
-
 __device__ __forceinline__ void store_row(const Args& a, int64_t pos, const Soft& s, const Result& q) {
-  const Soft one[1] = {s};
-  const Result res[1] = {q};
-  store_results<1>(a, pos, 0, one, res);
+  a.ent[pos] = q.ent;
+  if (a.labels) a.lp[pos] = q.lp;
+  if (a.stats) {
+    a.stats[pos] = s.m;
+    a.stats[a.positions + pos] = q.ls;
+    a.stats[2 * a.positions + pos] = q.ent;
+    a.stats[3 * a.positions + pos] = __int_as_float(a.labels ? q.label : -1);
+  }
 }
 
 // Short rows of adjacent classes: G lanes to a row, E packs of VEC classes to a lane, all of it in registers.  A
@@ -524,160 +498,147 @@ struct TopValues {
     }
   }
 };
-// Forward over strided classes: a thread has VEC positions of a line, UNR classes of them in registers at a time
-// (their loads are in flight together and the maximum's move costs one rescale).  With SPLIT the block's four waves
-// have the same 64 groups and a quarter of the classes each, joined through LDS: few positions still fill the card.
-template <typename T, int VEC, int K, bool SPLIT>
-__global__ __launch_bounds__(256) void probs_planes(const Args a, int64_t per_line, int64_t groups) {
-  constexpr int UNR = 8;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t want = SPLIT ? (int64_t)blockIdx.x * 64 + lane : (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const bool live = want < groups;
-  if (!SPLIT && !live) return;
-  const Group gr = group_of<VEC>(live ? want : groups - 1, per_line, a.n2);
-  const int64_t i0 = gr.line / a.n1, i1 = gr.line - i0 * a.n1;
-  const T* x = (const T*)a.x + i0 * a.s0 + i1 * a.s1 + gr.x0 * a.s2;
-  const uint8_t* mask = a.mask ? a.mask + (gr.pos / a.mask_div) * a.mask_stride : nullptr;
-  const int c0 = SPLIT ? (int)((int64_t)a.classes * wave >> 2) : 0;
-  const int c1 = SPLIT ? (int)((int64_t)a.classes * (wave + 1) >> 2) : a.classes;
-  int64_t y[VEC];
-  float xy[VEC];
-  if (!SPLIT || wave == 0) {
-    // the label's logit is fetched beside the loop, which reads its line as well
+// The classes that a mask row leaves in, in order, listed by the whole block: their number.
+constexpr int LIST = 4096;
+__device__ __forceinline__ int list_classes(const uint8_t* mask, int classes, uint16_t* list) {
+  __shared__ int before_wave[4];
+  const int per = (classes + 255) >> 8, c0 = threadIdx.x * per, c1 = min(classes, c0 + per);
+  int n = 0;
+  for (int c = c0; c < c1; ++c) n += mask[c] != 0;
+  int upto = n;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      y[j] = a.labels ? a.labels[gr.pos + j] : -1;
-      xy[j] = -INFINITY;
-    }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      if (y[j] >= 0 && y[j] < a.classes && !(mask && !mask[y[j]])) xy[j] = to_f(x[y[j] * a.sc + j * a.s2]);
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(upto, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) upto += v;
   }
-  Soft s[VEC];
-  TopValues<K> top[VEC];
-  bool nan[VEC];
+  if ((threadIdx.x & 63) == 63) before_wave[threadIdx.x >> 6] = upto;
+  __syncthreads();
+  int at = upto - n, all = 0;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) { s[j].clear(); top[j].clear(); nan[j] = false; }
-  auto chunk = [&](int c, const Pack<float, VEC> (&v)[UNR]) {
-    if constexpr (K > 0) {
+  for (int w = 0; w < 4; ++w) {
+    at += w < (int)(threadIdx.x >> 6) ? before_wave[w] : 0;
+    all += before_wave[w];
+  }
+  for (int c = c0; c < c1; ++c)
+    if (mask[c]) list[at++] = (uint16_t)c;
+  __syncthreads();
+  return all;
+}
+
+// How the positions lie over the blocks: `run` of them to each row of the class mask, in `blocks` blocks of their
+// own, so that a block's classes are one list (or one run of all)
+struct Tiling { int64_t run; unsigned blocks; };
+
+// Forward over strided classes: a thread has one position and UNR classes of it in registers at a time (their loads
+// are in flight together and the maximum's move costs one rescale); a wave reads 64 neighbours of each class plane.
+// With SPLIT the block's four waves have the same 64 positions and a quarter of the classes each, joined through
+// LDS: few positions still fill the card.  LISTED: only the planes of classes that the mask leaves in are read.
+template <typename T, int K, bool SPLIT, bool LISTED>
+__global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling tile) {
+  constexpr int UNR = 8;
+  __shared__ uint16_t list[LISTED ? LIST : 1];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const unsigned row = LISTED ? blockIdx.x / tile.blocks : 0;
+  const int64_t block = LISTED ? blockIdx.x - row * tile.blocks : blockIdx.x;
+  const int64_t want = SPLIT ? block * 64 + lane : block * 256 + threadIdx.x;
+  const bool live = want < tile.run;
+  int n = a.classes;
+  if (LISTED) n = list_classes(a.mask + row * a.mask_stride, a.classes, list);
+  if (!SPLIT && !live) return;
+  const int64_t pos = row * tile.run + (live ? want : tile.run - 1);
+  const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
+  const uint8_t* mask = a.mask ? a.mask + (LISTED ? row : pos / a.mask_div) * a.mask_stride : nullptr;
+  const int c0 = SPLIT ? (int)((int64_t)n * wave >> 2) : 0;
+  const int c1 = SPLIT ? (int)((int64_t)n * (wave + 1) >> 2) : n;
+  int64_t y = -1;
+  float xy = -INFINITY;
+  if (a.labels && (!SPLIT || wave == 0)) {
+    y = a.labels[pos];             // its logit is fetched beside the loop, which reads that line as well
+    if (y >= 0 && y < a.classes && !(mask && !mask[y])) xy = to_f(x[y * a.sc]);
+  }
+  Soft s;
+  s.clear();
+  TopValues<K> top;
+  top.clear();
+  bool nan = false;
+  auto chunk = [&](const int (&cls)[UNR], float (&f)[UNR]) {
 #pragma unroll
-      for (int u = 0; u < UNR; ++u) {
-        bool enter = false;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) enter |= v[u].v[j] > top[j].v[K - 1];
-        if (__any(enter))
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) top[j].add(v[u].v[j], c + u);
-      }
+    for (int u = 0; u < UNR; ++u) {
+      if constexpr (K > 0)
+        if (__any(f[u] > top.v[K - 1])) top.add(f[u], cls[u]);
+      nan |= f[u] != f[u];
     }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      float f[UNR];
-#pragma unroll
-      for (int u = 0; u < UNR; ++u) {
-        f[u] = v[u].v[j];
-        nan[j] |= f[u] != f[u];
-      }
-      s[j].template add_all<UNR>(f, a.c2);
-    }
+    s.template add_all<UNR>(f, a.c2);
   };
+  auto class_at = [&](int i) { return LISTED ? __builtin_amdgcn_readfirstlane((int)list[i]) : i; };
   int c = c0;
-  if (!mask)
+  if (LISTED || !mask)
     for (; c + UNR <= c1; c += UNR) {
-      Pack<T, VEC> v[UNR];
-      Pack<float, VEC> f[UNR];
+      T v[UNR];
+      float f[UNR];
+      int cls[UNR];
 #pragma unroll
-      for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + (c + u) * a.sc);
+      for (int u = 0; u < UNR; ++u) cls[u] = class_at(c + u);
 #pragma unroll
-      for (int u = 0; u < UNR; ++u)
+      for (int u = 0; u < UNR; ++u) v[u] = x[cls[u] * a.sc];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[u].v[j] = to_f(v[u].v[j]);
-      chunk(c, f);
+      for (int u = 0; u < UNR; ++u) f[u] = to_f(v[u]);
+      chunk(cls, f);
     }
   for (; c < c1; c += UNR) {
-    Pack<T, VEC> v[UNR];
-    Pack<float, VEC> f[UNR];
+    T v[UNR];
+    float f[UNR];
+    int cls[UNR];
     bool in[UNR];
 #pragma unroll
     for (int u = 0; u < UNR; ++u) {
-      const int cu = min(c + u, c1 - 1);
-      v[u] = load_pack<T, VEC>(x + cu * a.sc);
-      in[u] = c + u < c1 && (!mask || mask[cu]);
+      cls[u] = class_at(min(c + u, c1 - 1));
+      v[u] = x[cls[u] * a.sc];
+      in[u] = c + u < c1 && (LISTED || !mask || mask[cls[u]]);
     }
 #pragma unroll
-    for (int u = 0; u < UNR; ++u)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[u].v[j] = in[u] ? to_f(v[u].v[j]) : -INFINITY;
-    chunk(c, f);
+    for (int u = 0; u < UNR; ++u) f[u] = in[u] ? to_f(v[u]) : -INFINITY;
+    chunk(cls, f);
   }
   if constexpr (SPLIT) {
-    __shared__ Soft part[4][64 * VEC];
-    __shared__ bool part_nan[4][64 * VEC];
-    __shared__ TopValues<K> part_top[K > 0 ? 4 : 1][K > 0 ? 64 * VEC : 1];
-    if (wave)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        part[wave][j * 64 + lane] = s[j];
-        part_nan[wave][j * 64 + lane] = nan[j];
-        if constexpr (K > 0) part_top[wave][j * 64 + lane] = top[j];
-      }
+    __shared__ Soft part[4][64];
+    __shared__ bool part_nan[4][64];
+    __shared__ TopValues<K> part_top[K > 0 ? 4 : 1][K > 0 ? 64 : 1];
+    if (wave) {
+      part[wave][lane] = s;
+      part_nan[wave][lane] = nan;
+      if constexpr (K > 0) part_top[wave][lane] = top;
+    }
     __syncthreads();
     if (wave || !live) return;
+#pragma unroll 1
+    for (int w = 1; w < 4; ++w) {
+      s.join(part[w][lane], a.c2);
+      nan |= part_nan[w][lane];
+      if constexpr (K > 0)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      for (int w = 1; w < 4; ++w) {
-        s[j].join(part[w][j * 64 + lane], a.c2);
-        nan[j] |= part_nan[w][j * 64 + lane];
-        if constexpr (K > 0)
-#pragma unroll
-          for (int i = 0; i < K; ++i) top[j].add(part_top[w][j * 64 + lane].v[i], part_top[w][j * 64 + lane].id[i]);
-      }
+        for (int i = 0; i < K; ++i) top.add(part_top[w][lane].v[i], part_top[w][lane].id[i]);
+    }
   }
-  Result q[VEC];
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) q[j] = result_of(a, s[j], nan[j], y[j], xy[j]);
-  store_results<VEC>(a, gr.pos, gr.skip, s, q);
+  const Result q = result_of(a, s, nan, y, xy);
+  store_row(a, pos, s, q);
   if constexpr (K > 0) {
-    // positions behind the class dim: a line lies in one of their runs, or there are none
-    const int64_t o = a.inner == 1 ? gr.pos : gr.pos / a.inner;
-#pragma unroll
-    for (int i = 0; i < K; ++i)
-      if (i < a.k) {
-        Pack<float, VEC> lp;
-        Pack<int, VEC> id;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          id.v[j] = top[j].id[i];
-          lp.v[j] = id.v[j] < 0 ? -INFINITY : (top[j].v[i] - s[j].m) * a.inv_t - q[j].ls;
-        }
-        if (a.inner == 1) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            if (j >= gr.skip) {
-              a.top_lp[(gr.pos + j) * a.k + i] = lp.v[j];
-              a.top_id[(gr.pos + j) * a.k + i] = id.v[j];
-            }
-        } else {
-          const int64_t at = (o * a.k + i) * a.inner + gr.pos - o * a.inner;
-          store_own<VEC>(a.top_lp + at, lp, gr.skip);
-          store_own<VEC>(a.top_id + at, id, gr.skip);
-        }
-      }
-    // a position that has NaNs (all its values are): those classes first, lower class first, then by value
-    int redo = 0;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) redo |= nan[j] && j >= gr.skip ? 1 << j : 0;
-    for (; redo; redo &= redo - 1) {
-      const int j = __ffs(redo) - 1;
+    const int64_t o = a.inner == 1 ? pos : pos / a.inner, at = o * a.k * a.inner + pos - o * a.inner;
+    if (nan) {
+      // every value is NaN: the classes that are come first, lower class first, then the others by value
       Top<K> keys;
       keys.clear();
       for (int k = 0; k < a.classes; ++k)
-        if (!mask || mask[k]) keys.add(order_key(to_f(x[k * a.sc + j * a.s2])), k);
-      const int64_t at = o * a.k * a.inner + (a.inner == 1 ? j * a.k : gr.pos - o * a.inner + j);
+        if (!mask || mask[k]) keys.add(order_key(to_f(x[k * a.sc])), k);
 #pragma unroll
-      for (int i = 0; i < K; ++i)
-        if (i < a.k) a.top_id[at + i * a.inner] = keys.id[i];
+      for (int i = 0; i < K; ++i) top.id[i] = keys.id[i];
     }
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+      if (i < a.k) {
+        a.top_lp[at + i * a.inner] = top.id[i] < 0 ? -INFINITY : (top.v[i] - s.m) * a.inv_t - q.ls;
+        a.top_id[at + i * a.inner] = top.id[i];
+      }
   }
 }
 
@@ -716,30 +677,44 @@ __device__ __forceinline__ float grad_of(const BwdArgs<T>& a, const RowGrad& g, 
   return (c == g.label ? g.gl : 0.f) - p * w;
 }
 
-// Backward over strided classes: a thread has VEC positions of a line and `span` classes, so that a wave reads
-// and writes whole stretches of a class plane.
-template <typename T, int VEC>
-__global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, int64_t per_line, int64_t groups,
-                                                        int span) {
-  const int64_t gi = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (gi >= groups) return;
-  const Group gr = group_of<VEC>(gi, per_line, a.n2);
-  const int64_t i0 = gr.line / a.n1, i1 = gr.line - i0 * a.n1;
-  const T* x = a.x + i0 * a.s0 + i1 * a.s1 + gr.x0 * a.s2;
-  T* dx = a.dx + i0 * a.o0 + i1 * a.o1 + gr.x0 * a.o2;
-  const uint8_t* mask = a.mask ? a.mask + (gr.pos / a.mask_div) * a.mask_stride : nullptr;
-  RowGrad g[VEC];
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) g[j] = row_grad(a, gr.pos + j);
+// Backward over strided classes: a thread has one position and `span` <= 64 classes, a wave reads and writes 64
+// neighbours of each class plane.  UNIFORM: a block's positions share a row of the class mask, whose bits for the
+// span every wave gathers once; planes that it leaves out are not read.
+template <typename T, bool UNIFORM>
+__global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, const Tiling tile, int span) {
+  constexpr int UNR = 8;
+  const unsigned row = UNIFORM ? blockIdx.x / tile.blocks : 0;
+  const int64_t want = (int64_t)(UNIFORM ? blockIdx.x - row * tile.blocks : blockIdx.x) * 256 + threadIdx.x;
   const int c0 = blockIdx.y * span, c1 = min(a.classes, c0 + span);
-#pragma unroll 4
-  for (int c = c0; c < c1; ++c) {
-    const Pack<T, VEC> v = load_pack<T, VEC>(x + c * a.sc);
-    const bool out = mask && !mask[c];
-    Pack<T, VEC> d;
+  uint64_t bits = ~0ull;
+  if (UNIFORM) {
+    const int c = c0 + (int)(threadIdx.x & 63);
+    bits = __ballot(c < c1 && a.mask[row * a.mask_stride + c]);
+  }
+  if (want >= tile.run) return;
+  const int64_t pos = row * tile.run + want;
+  const T* x = a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
+  T* dx = a.dx + offset_of(pos, a.n1, a.n2, a.o0, a.o1, a.o2);
+  const uint8_t* mask = !UNIFORM && a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
+  T v[UNR];
+  auto load = [&](int c) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) d.v[j] = from_f<T>(out ? 0.f : grad_of(a, g[j], to_f(v.v[j]), c));
-    store_own<VEC>(dx + c * a.oc, d, gr.skip);
+    for (int u = 0; u < UNR; ++u) {
+      const int cu = min(c + u, c1 - 1);
+      if (!UNIFORM || bits >> (cu - c0) & 1) v[u] = x[cu * a.sc];
+    }
+  };
+  load(c0);                        // under way before what the position's sums need
+  const RowGrad g = row_grad(a, pos);
+  for (int c = c0; c < c1; c += UNR) {
+    if (c > c0) load(c);
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) {
+      const int cu = c + u;
+      if (cu >= c1) break;
+      const bool in = UNIFORM ? bits >> (cu - c0) & 1 : !mask || mask[cu];
+      dx[cu * a.oc] = from_f<T>(in ? grad_of(a, g, to_f(v[u]), cu) : 0.f);
+    }
   }
 }
 
@@ -791,31 +766,46 @@ bool bad_positions(int64_t n0, int64_t n1, int64_t n2, int64_t classes, int64_t*
   return *n > (1LL << 38);                      // grids stay below 2^31 blocks of 256
 }
 
-template <typename T, int VEC, int K>
-void launch_planes_as(const Args& a, hipStream_t s) {
-  const int64_t per_line = (a.n2 + VEC - 1) / VEC, groups = a.positions / a.n2 * per_line;
-  // four waves to a group where whole groups would leave the card with less than 8 waves a CU
-  if (groups < 64 * 2048 && a.classes >= 16)
-    hipLaunchKernelGGL((probs_planes<T, VEC, K, true>), dim3((unsigned)((groups + 63) / 64)), dim3(256), 0, s, a,
-                       per_line, groups);
-  else
-    hipLaunchKernelGGL((probs_planes<T, VEC, K, false>), dim3((unsigned)((groups + 255) / 256)), dim3(256), 0, s, a,
-                       per_line, groups);
+// whether whole blocks of positions can share a row of the class mask, and the runs then
+bool mask_runs(const void* mask, int64_t mask_div, int64_t positions, int per_block, Tiling* t, int64_t* rows) {
+  t->run = positions;
+  *rows = 1;
+  if (mask && mask_div < positions) {
+    if (mask_div < 64) return false;
+    t->run = mask_div;
+    *rows = (positions + mask_div - 1) / mask_div;
+  }
+  t->blocks = (unsigned)((t->run + per_block - 1) / per_block);
+  return mask != nullptr;
 }
-template <typename T, int VEC>
-void launch_planes_top(const Args& a, hipStream_t s) {
-  if (a.k == 0) launch_planes_as<T, VEC, 0>(a, s);
-  else if (a.k == 1) launch_planes_as<T, VEC, 1>(a, s);
-  else if (a.k == 2) launch_planes_as<T, VEC, 2>(a, s);
-  else if (a.k <= 4) launch_planes_as<T, VEC, 4>(a, s);
-  else if (a.k <= 8) launch_planes_as<T, (VEC > 2 ? 2 : VEC), 8>(a, s);
-  else launch_planes_as<T, 1, 16>(a, s);
+
+template <typename T, int K, bool SPLIT>
+void launch_planes_as(const Args& a, hipStream_t s) {
+  constexpr int PER = SPLIT ? 64 : 256;
+  Tiling t;
+  int64_t rows;
+  if (a.classes <= LIST && mask_runs(a.mask, a.mask_div, a.positions, PER, &t, &rows)) {
+    hipLaunchKernelGGL((probs_planes<T, K, SPLIT, true>), dim3((unsigned)(rows * t.blocks)), dim3(256), 0, s, a, t);
+  } else {
+    t.run = a.positions;
+    t.blocks = (unsigned)((t.run + PER - 1) / PER);
+    hipLaunchKernelGGL((probs_planes<T, K, SPLIT, false>), dim3(t.blocks), dim3(256), 0, s, a, t);
+  }
+}
+template <typename T, int K>
+void launch_planes_split(const Args& a, hipStream_t s) {
+  // four waves to 64 positions where whole ones would leave the card with less than 8 waves a CU
+  if (a.positions < 64 * 2048 && a.classes >= 16) launch_planes_as<T, K, true>(a, s);
+  else launch_planes_as<T, K, false>(a, s);
 }
 template <typename T>
 int launch_planes(const Args& a, hipStream_t s) {
-  const bool lines = a.s2 == 1 && !(a.mask && a.mask_div % a.n2);
-  if (lines && a.n2 >= 4 && a.positions >= 4 * 64 * 512) launch_planes_top<T, 4>(a, s);
-  else launch_planes_top<T, 1>(a, s);
+  if (a.k == 0) launch_planes_split<T, 0>(a, s);
+  else if (a.k == 1) launch_planes_split<T, 1>(a, s);
+  else if (a.k == 2) launch_planes_split<T, 2>(a, s);
+  else if (a.k <= 4) launch_planes_split<T, 4>(a, s);
+  else if (a.k <= 8) launch_planes_split<T, 8>(a, s);
+  else launch_planes_split<T, 16>(a, s);
   LDM_CHECK_LAUNCH();
   return LDM_OK;
 }
@@ -902,15 +892,20 @@ int launch_bwd(const ldm_label_probs_bwd_params* p, int64_t n, hipStream_t s) {
     LDM_CHECK_LAUNCH();
     return LDM_OK;
   }
-  const bool wide = p->s2 == 1 && p->o2 == 1 && p->n2 >= 4 && !(a.mask && a.mask_div % p->n2);
-  const int vec = wide ? 4 : 1;
-  const int64_t per_line = (p->n2 + vec - 1) / vec, groups = n / p->n2 * per_line, blocks = (groups + 255) / 256;
-  int span = a.classes;                          // 8 classes at least to a thread, 2048 blocks where there is work
-  while (span > 8 && blocks * ((a.classes + span - 1) / span) < 2048) span = (span + 1) / 2;
-  span = std::max(span, (a.classes + 65534) / 65535);
-  const dim3 grid((unsigned)blocks, (unsigned)((a.classes + span - 1) / span));
-  if (wide) hipLaunchKernelGGL((probs_bwd_planes<T, 4>), grid, dim3(256), 0, s, a, per_line, groups, span);
-  else hipLaunchKernelGGL((probs_bwd_planes<T, 1>), grid, dim3(256), 0, s, a, per_line, groups, span);
+  // 32 classes to a thread, or down to 8 where the card would have less than 12 waves a CU
+  int span = 32;
+  while (span > 8 && n / 64 * ((a.classes + span - 1) / span) < 12 * 256) span /= 2;
+  const unsigned spans = (unsigned)((a.classes + span - 1) / span);
+  if (spans > 65535) return LDM_ERR_ARG;
+  Tiling t;
+  int64_t rows;
+  if (mask_runs(a.mask, a.mask_div, n, 256, &t, &rows)) {
+    hipLaunchKernelGGL((probs_bwd_planes<T, true>), dim3((unsigned)(rows * t.blocks), spans), dim3(256), 0, s, a, t, span);
+  } else {
+    t.run = n;
+    t.blocks = (unsigned)((n + 255) / 256);
+    hipLaunchKernelGGL((probs_bwd_planes<T, false>), dim3(t.blocks, spans), dim3(256), 0, s, a, t, span);
+  }
   LDM_CHECK_LAUNCH();
   return LDM_OK;
 }
