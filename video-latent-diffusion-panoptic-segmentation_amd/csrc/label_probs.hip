@@ -167,38 +167,63 @@ __device__ __forceinline__ int64_t offset_of(int64_t pos, int64_t n1, int64_t n2
   return (line / n1) * s0 + (line % n1) * s1 + (pos % n2) * s2;
 }
 
+// Reductions by DPP, in the vector pipe; a shuffle is a trip through LDS.
+// Over G = 1 .. 64 neighbouring lanes, in each of them: quads, then mirrored halves of 8 and 16, then rows of 16.
+template <int CTRL, typename V> __device__ __forceinline__ V dpp(V v) {
+  return __builtin_bit_cast(V, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int G, typename V, typename F> __device__ __forceinline__ V lanes_join(V v, F f) {
+  if constexpr (G >= 2) v = f(v, dpp<0xB1>(v));      // quad_perm 1 0 3 2
+  if constexpr (G >= 4) v = f(v, dpp<0x4E>(v));      // quad_perm 2 3 0 1
+  if constexpr (G >= 8) v = f(v, dpp<0x141>(v));     // row_half_mirror
+  if constexpr (G >= 16) v = f(v, dpp<0x140>(v));    // row_mirror
+  if constexpr (G >= 32) v = f(v, __shfl_xor(v, 16, 64));
+  if constexpr (G >= 64) v = f(v, __shfl_xor(v, 32, 64));
+  return v;
+}
+// Over the wave, as a scalar: rows of 16 as above, then the row totals to the last lane.  `none` changes nothing.
+template <typename V, typename F> __device__ __forceinline__ V wave_all(V v, V none, F f) {
+  v = lanes_join<16>(v, f);
+  const int n = __builtin_bit_cast(int, none);
+  v = f(v, __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(n, __builtin_bit_cast(int, v), 0x142, 0xa, 0xf, false)));
+  v = f(v, __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(n, __builtin_bit_cast(int, v), 0x143, 0xc, 0xf, false)));
+  return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+struct Max {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+  __device__ __forceinline__ int operator()(int a, int b) const { return max(a, b); }
+};
+struct Min { __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return min(a, b); } };
+
 // the wave's Softs joined, in every lane
 __device__ __forceinline__ Soft wave_join(const Soft& s, float c2) {
-  const float m = wave_max(s.m), to = m == -INFINITY ? 0.f : m;
+  const float m = wave_all(s.m, -INFINITY, Max()), to = m == -INFINITY ? 0.f : m;
   const bool holds = s.m == m;     // the first lane that holds the maximum keeps its term out of the sums
   const bool keeper = holds && (int)(threadIdx.x & 63) == __ffsll((unsigned long long)__ballot(holds)) - 1;
   Soft o = s;
   o.rescale(to, c2);
   const float d = fmaxf(s.m - to, LOWEST), e = keeper ? 0.f : exp2_fast(d * c2);
   o.m = m;
-  o.r = wave_sum(o.r + e);
-  o.t = wave_sum(fmaf(d, e, o.t));
+  o.r = wave_all(o.r + e, 0.f, Add());
+  o.t = wave_all(fmaf(d, e, o.t), 0.f, Add());
   return o;
 }
 
-// (key, class) pairs in the order of the answer: larger key, then lower class; an empty one (-1) last
-__device__ __forceinline__ bool before(int k, int c, int key, int id) {
-  return k > key || (k == key && (unsigned)c < (unsigned)id);
-}
-// the n first of the wave's lists: lane j < n gets the j-th
+// the n first of the wave's lists, larger key, then lower class: lane j < n gets the j-th
 template <int K>
 __device__ __forceinline__ void wave_top(Top<K>& top, int n, int& key, int& id) {
   key = KEY_NONE;
   id = -1;
   for (int j = 0; j < n; ++j) {
-    int k = top.key[0], c = top.id[0];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const int k2 = __shfl_xor(k, o, 64), c2 = __shfl_xor(c, o, 64);
-      if (before(k2, c2, k, c)) { k = k2; c = c2; }
-    }
+    const int k = wave_all(top.key[0], KEY_NONE, Max());
+    const bool holds = top.key[0] == k;
+    const unsigned long long who = __ballot(holds);
+    int c = __builtin_amdgcn_readlane(top.id[0], __ffsll(who) - 1);
+    if (who & (who - 1)) c = (int)wave_all(holds ? (unsigned)top.id[0] : ~0u, ~0u, Min());
+    if (c < 0) break;
     if ((int)(threadIdx.x & 63) == j) { key = k; id = c; }
-    if (top.id[0] == c && c >= 0) {
+    if (holds && top.id[0] == c) {
 #pragma unroll
       for (int i = 0; i + 1 < K; ++i) { top.key[i] = top.key[i + 1]; top.id[i] = top.id[i + 1]; }
       top.key[K - 1] = KEY_NONE;
@@ -241,16 +266,6 @@ __device__ __forceinline__ void store_row(const Args& a, int64_t pos, const Soft
 
 // Short rows of adjacent classes: G lanes to a row, E packs of VEC classes to a lane, all of it in registers.  A
 // row's last pack reaches back over its neighbour; the classes it has in common with it count once.
-template <int G> __device__ __forceinline__ float lanes_max(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
-template <int G> __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
 template <typename T, int VEC, int G, int E, bool TOP>
 __global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
   constexpr int N = VEC * E;
@@ -292,7 +307,7 @@ __global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
     hi = fmaxf(hi, w);
   }
   Soft s;
-  s.m = lanes_max<G>(hi);
+  s.m = lanes_join<G>(hi, Max());
   const float to = s.m == -INFINITY ? 0.f : s.m;
   const uint64_t mine = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1)) << (lane & ~(G - 1));
   const uint64_t holds = __ballot(hi == s.m) & mine;
@@ -306,8 +321,8 @@ __global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
     r += e;
     t = fmaf(d, e, t);
   }
-  s.r = lanes_sum<G>(r);
-  s.t = lanes_sum<G>(t);
+  s.r = lanes_join<G>(r, Add());
+  s.t = lanes_join<G>(t, Add());
   const Result q = result_of(a, s, nan, y, xy);
   if (live && sub == 0) store_row(a, pos, s, q);
   if constexpr (TOP) {
@@ -318,11 +333,9 @@ __global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
         const int ci = min((sub + i / VEC * G) * VEC, a.classes - VEC) + i % VEC;
         if (key[i] > k) { k = key[i]; c = ci; }
       }
-#pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) {
-        const int k2 = __shfl_xor(k, o, 64), c2 = __shfl_xor(c, o, 64);
-        if (before(k2, c2, k, c)) { k = k2; c = c2; }
-      }
+      const int best = lanes_join<G>(k, Max());
+      c = (int)lanes_join<G>(k == best ? (unsigned)c : ~0u, Min());
+      k = best;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int ci = min((sub + i / VEC * G) * VEC, a.classes - VEC) + i % VEC;
@@ -367,14 +380,21 @@ __device__ __forceinline__ bool block_join_row(RowParts<K>& sh, Soft& s, Top<K>&
   }
   return true;
 }
+// a row's label and its logit (-inf where it is no class or is masked): fetched first, needed last
+struct LabelAt { int64_t y; float xy; };
 template <typename T>
-__device__ __forceinline__ void finish_row(const Args& a, int64_t pos, const Soft& s, bool nan, int key, int id) {
+__device__ __forceinline__ LabelAt label_at(const Args& a, int64_t pos) {
+  LabelAt r = {-1, -INFINITY};
+  if (!a.labels) return r;
+  r.y = a.labels[pos];
+  if (r.y >= 0 && r.y < a.classes && !(a.mask && !a.mask[(pos / a.mask_div) * a.mask_stride + r.y]))
+    r.xy = to_f(((const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2))[r.y]);
+  return r;
+}
+__device__ __forceinline__ void finish_row(const Args& a, int64_t pos, const LabelAt& l, const Soft& s, bool nan, int key,
+                                           int id) {
   const int lane = threadIdx.x & 63;
-  const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
-  const int64_t y = a.labels ? a.labels[pos] : -1;
-  float xy = -INFINITY;
-  if (y >= 0 && y < a.classes && !(a.mask && !a.mask[(pos / a.mask_div) * a.mask_stride + y])) xy = to_f(x[y]);
-  const Result q = result_of(a, s, nan, y, xy);
+  const Result q = result_of(a, s, nan, l.y, l.xy);
   if (lane == 0) store_row(a, pos, s, q);
   if (lane < a.k) store_top(a, pos, lane, key, id, s, q.ls);
 }
@@ -395,6 +415,8 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
   Top<K> top;
   top.clear();
   bool nan = false;
+  LabelAt l;
+  if (segments == 1) l = label_at<T>(a, pos);
   int bar = KEY_NONE;              // the wave's lists hold K keys that are no less
   for (int base = seg * seg_len; base < end; base += 256 * N) {   // the same turns in every lane: they shuffle
     const int at0 = base + tid * VEC;
@@ -428,9 +450,7 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
           const int k = order_key(f[i]);
           if (k > bar) top.add(k, min(at0 + i / VEC * 256 * VEC, last) + i % VEC);
         }
-        bar = top.key[K - 1];
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) bar = max(bar, __shfl_xor(bar, o, 64));
+        bar = wave_all(top.key[K - 1], KEY_NONE, Max());
       }
     }
     s.template add_all<N>(f, a.c2);
@@ -438,7 +458,7 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
   int key = KEY_NONE, id = -1;
   if (!block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) return;
   if (segments == 1) {
-    finish_row<T>(a, pos, s, nan, key, id);
+    finish_row(a, pos, l, s, nan, key, id);
     return;
   }
   if (lane == 0) parts[blockIdx.x] = {s.m, s.r, s.t, nan};
@@ -456,20 +476,24 @@ __global__ __launch_bounds__(256) void probs_join(const Args a, int segments, co
   Top<K> top;
   top.clear();
   bool nan = false;
+  const LabelAt l = label_at<T>(a, pos);
   for (int i = threadIdx.x; i < segments; i += 256) {
     const Part p = parts[pos * segments + i];
+    int2 kc[K > 0 ? K : 1];
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (j < a.k) kc[j] = part_top[(pos * segments + i) * a.k + j];
     Soft o;
     o.m = p.m; o.r = p.r; o.t = p.t;
     s.join(o, a.c2);
     nan |= p.nan != 0;
     if constexpr (K > 0)
-      for (int j = 0; j < a.k; ++j) {
-        const int2 kc = part_top[(pos * segments + i) * a.k + j];
-        if (kc.y >= 0) top.add(kc.x, kc.y);
-      }
+#pragma unroll
+      for (int j = 0; j < K; ++j)
+        if (j < a.k && kc[j].y >= 0) top.add(kc[j].x, kc[j].y);
   }
   int key = KEY_NONE, id = -1;
-  if (block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) finish_row<T>(a, pos, s, nan, key, id);
+  if (block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) finish_row(a, pos, l, s, nan, key, id);
 }
 
 // What a thread of probs_planes keeps of the most likely classes of one position: values in falling order.  A new
