@@ -137,7 +137,8 @@ def test_strided_positions_address_every_element(make, dim):
     base = torch.arange(2 * 5 * 6 * 8).view(2, 5, 6, 8)
     x = make(base)
     dim = dim % x.ndim
-    y, n, s, N, inner, out, o = K._label_positions(x, dim, grad=True)
+    y, n, s, inner, out, o = K._label_positions(x, dim, torch.empty_like(x))
+    N = n[0] * n[1] * n[2]
     idx = [torch.arange(k) for k in n]
     grid = sum(i.view([-1 if j == d else 1 for j in range(3)]) * st for d, (i, st) in enumerate(zip(idx, s)))
     want = x.movedim(dim, 0).reshape(x.shape[dim], -1)

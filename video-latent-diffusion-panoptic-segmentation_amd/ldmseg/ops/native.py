@@ -10,7 +10,9 @@ import collections
 import contextlib
 import ctypes
 import math
+import operator
 import os
+import struct
 import threading
 
 import torch
@@ -193,9 +195,9 @@ EXPORTS = {
     "ldm_space_to_depth2": (_i, [_vp, _i, _i, _i, _i, _vp, _i, _vp]),
     "ldm_posterior_sample": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp]),
     "ldm_posterior_bwd": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
-    "ldm_label_log_probs_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LabelProbsParams)]),
-    "ldm_label_log_probs": (_i, [ctypes.POINTER(LabelProbsParams), _vp]),
-    "ldm_label_log_probs_bwd": (_i, [ctypes.POINTER(LabelProbsBwdParams), _vp]),
+    "ldm_label_log_probs_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "ldm_label_log_probs": (_i, [_vp, _vp]),
+    "ldm_label_log_probs_bwd": (_i, [_vp, _vp]),
     "ldm_grad_norm_workspace_bytes": (ctypes.c_size_t, [_vp, _i]),
     "ldm_grad_norm": (_i, [_vp, _vp, _vp, _i, _i, _d, _i, _vp, _vp, _i64, _vp]),
     "ldm_status_string": (ctypes.c_char_p, [_i]),
@@ -259,12 +261,17 @@ def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
-_HERE = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda i: torch.cuda.current_stream(i).cuda_stream
 
 
-def _on_device(dev):
-    """Context in which launches go to ``dev`` (nothing to do where it is the current device)."""
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _launch(dev, fn, *args):
+    """fn(*args, stream) with ``dev`` as the current device, on its current stream."""
+    i = dev.index
+    if i == torch.cuda.current_device():
+        return fn(*args, _raw_stream(i))
+    with torch.cuda.device(i):
+        return fn(*args, _raw_stream(i))
 
 
 def _contig(t, name):
@@ -1876,6 +1883,12 @@ def posterior_bwd(moments, eps, dz_nhwc):
 LABEL_TOPK_MAX = 16
 LabelProbs = collections.namedtuple("LabelProbs", "log_prob entropy top_log_probs top_ids stats")
 
+# LabelProbsParams / LabelProbsBwdParams as bytes (a ctypes.Structure takes several times as long to fill)
+_LABEL_PARAMS = struct.Struct("@22qf3i")
+_LABEL_BWD_PARAMS = struct.Struct("@20qfi")
+assert _LABEL_PARAMS.size == ctypes.sizeof(LabelProbsParams)
+assert _LABEL_BWD_PARAMS.size == ctypes.sizeof(LabelProbsBwdParams)
+
 
 def _merge_dims(sizes, *strides):
     """(sizes, strides...) without dims of size 1 and with adjacent dims merged where every layout has them
@@ -1895,32 +1908,39 @@ def _merge_dims(sizes, *strides):
     return ns, out
 
 
-def _label_positions(x, dim, grad=False):
-    """The positions of ``x`` (every dim but ``dim``) as up to three strided dims: (x, sizes, strides,
-    n_positions, inner, out, out strides).  ``inner`` counts the positions behind the class dim; dims are
-    merged on either side of it, never across it, and a tensor with more than three left is copied.  With
-    ``grad``, ``out`` is an uninitialised tensor like x, walked by the same sizes."""
+def _label_positions(x, dim, out=None):
+    """The positions of ``x`` (every dim but ``dim``) as three strided dims: (x, sizes, strides, positions behind
+    the class dim, out, out's strides).  Dims are merged on either side of the class dim, never across it; a tensor
+    with more than three left is copied.  ``out``: a tensor like x that is walked by the same sizes."""
+    shape = x.shape
     if x.is_contiguous():
-        inner = math.prod(x.shape[dim + 1:])
-        outer = math.prod(x.shape[:dim])
-        s = (0, x.shape[dim] * inner, 1)
-        return x, (1, outer, inner), s, outer * inner, inner, torch.empty_like(x) if grad else None, s
-    out = torch.empty_like(x) if grad else None
-    layouts = [x.stride()] + ([out.stride()] if grad else [])
-    no, so = _merge_dims(x.shape[:dim], *[st[:dim] for st in layouts])
-    ni, si = _merge_dims(x.shape[dim + 1:], *[st[dim + 1:] for st in layouts])
+        inner = math.prod(shape[dim + 1:])
+        s = (0, shape[dim] * inner, 1)
+        return x, (1, math.prod(shape[:dim]), inner), s, inner, out, s
+    st = x.stride()
+    if dim == 1:
+        so = st if out is None else out.stride()
+        if x.ndim == 4 and 1 not in shape:
+            n, h, w = shape[0], shape[2], shape[3]
+            if st[2] == w * st[3] and so[2] == w * so[3]:
+                return x, (1, n, h * w), (0, st[0], st[3]), h * w, out, (0, so[0], so[3])
+            return x, (n, h, w), (st[0], st[2], st[3]), h * w, out, (so[0], so[2], so[3])
+        if x.ndim == 2:
+            return x, (1, 1, shape[0]), (0, 0, st[0]), 1, out, (0, 0, so[0])
+    layouts = [st] if out is None else [st, out.stride()]
+    no, so = _merge_dims(shape[:dim], *[t[:dim] for t in layouts])
+    ni, si = _merge_dims(shape[dim + 1:], *[t[dim + 1:] for t in layouts])
     n = no + ni
     if len(n) > 3:
-        return _label_positions(x.contiguous(), dim, grad)
+        x = x.contiguous()
+        return _label_positions(x, dim, None if out is None else torch.empty_like(x))
     pad = 3 - len(n)
     s = [[0] * pad + a + b for a, b in zip(so, si)]
-    return x, [1] * pad + n, s[0], math.prod(n), math.prod(ni), out, s[-1]
+    return x, [1] * pad + n, s[0], math.prod(ni), out, s[-1]
 
 
 def _label_mask(class_mask, logits, dim, n_positions):
     """(mask, row stride, positions to a row) of a class mask [C] or [logits.shape[0], C]."""
-    if class_mask is None:
-        return None, 0, 1
     C, B = logits.shape[dim], logits.shape[0]
     if class_mask.dtype != torch.bool or class_mask.device != logits.device:
         raise TypeError("class_mask must be a bool tensor on the logits' device")
@@ -1932,21 +1952,21 @@ def _label_mask(class_mask, logits, dim, n_positions):
                      f"{tuple(class_mask.shape)}")
 
 
-def _label_dim(logits, dim):
-    if logits.ndim < 2:
+def _label_checked(logits, dim, temperature):
+    """(class dim, positions' shape, dtype code) of checked arguments."""
+    code = dtype_code(logits.dtype)
+    nd = logits.ndim
+    if nd < 2:
         raise ValueError("logits need a class dim and at least one position dim")
-    d = dim + logits.ndim if dim < 0 else dim
-    if not 0 <= d < logits.ndim:
-        raise ValueError(f"class dim {dim} is outside logits of {logits.ndim} dims")
-    if logits.shape[d] == 0:
+    if not -nd <= dim < nd:
+        raise ValueError(f"class dim {dim} is outside logits of {nd} dims")
+    dim %= nd
+    shape = logits.shape
+    if shape[dim] == 0:
         raise ValueError("logits have no classes")
-    return d
-
-
-def _label_temperature(t):
-    if not 1e-4 <= t <= 1e4:
-        raise ValueError(f"temperature must be in [1e-4, 1e4], got {t}")
-    return float(t)
+    if not 1e-4 <= temperature <= 1e4:
+        raise ValueError(f"temperature must be in [1e-4, 1e4], got {temperature}")
+    return dim, shape[:dim] + shape[dim + 1:], code
 
 
 def label_log_probs(logits, labels=None, *, dim=1, topk=0, temperature=1.0, ignore_label=None, class_mask=None,
@@ -1966,53 +1986,50 @@ def label_log_probs(logits, labels=None, *, dim=1, topk=0, temperature=1.0, igno
     ``class_mask`` (bool [C] or [logits.shape[0], C]) leaves classes out whatever their logits hold.  A row
     that is left without a class has entropy 0 and no alternatives; a NaN or +inf among the classes left
     makes the row's log_prob and entropy NaN."""
-    code = dtype_code(logits.dtype)
-    dim = _label_dim(logits, dim)
-    temperature = _label_temperature(temperature)
-    shape = logits.shape
-    C = shape[dim]
-    pos_shape = shape[:dim] + shape[dim + 1:]
+    dim, pos_shape, code = _label_checked(logits, dim, temperature)
+    C = logits.shape[dim]
     if not 0 <= topk <= min(C, LABEL_TOPK_MAX):
         raise ValueError(f"topk must be in [0, {min(C, LABEL_TOPK_MAX)}], got {topk}")
     dev = logits.device
+    y = lp = top_lp = top_id = stats = None
     if labels is not None:
         if labels.dtype != torch.int64 or labels.device != dev:
             raise TypeError("labels must be an int64 tensor on the logits' device")
         if labels.shape != pos_shape:
             raise ValueError(f"labels must be {tuple(pos_shape)}, got {tuple(labels.shape)}")
-        labels = labels.contiguous()
+        y = labels.contiguous()
     N = math.prod(pos_shape)
-    mask, mask_stride, mask_div = _label_mask(class_mask, logits, dim, N)
+    mask, mask_stride, mask_div = (None, 0, 1) if class_mask is None else _label_mask(class_mask, logits, dim, N)
     _gpu(logits)
-    lib = load_library()
-    x, n, s, _, inner, _, _ = _label_positions(logits, dim)
+    lib = _lib or load_library()
+    x, n, s, inner, _, _ = _label_positions(logits, dim)
     entropy = torch.empty(pos_shape, dtype=torch.float32, device=dev)
-    log_prob = None if labels is None else torch.empty_like(entropy)
-    top_lp = top_id = stats = None
+    if y is not None:
+        lp = torch.empty_like(entropy)
     if topk:
-        top_shape = shape[:dim] + (topk,) + shape[dim + 1:]
-        top_lp = torch.empty(top_shape, dtype=torch.float32, device=dev)
-        top_id = torch.empty(top_shape, dtype=torch.int32, device=dev)
+        top_lp = entropy.new_empty(logits.shape[:dim] + (topk,) + logits.shape[dim + 1:])
+        top_id = torch.empty_like(top_lp, dtype=torch.int32)
     if want_stats:
-        stats = torch.empty((4,) + pos_shape, dtype=torch.float32, device=dev)
+        stats = entropy.new_empty((4,) + pos_shape)
     if N:
-        p = LabelProbsParams(x.data_ptr(), *n, *s, C, x.stride(dim), _ptr(labels),
-                             0 if ignore_label is None else int(ignore_label), _ptr(mask), mask_stride, mask_div,
-                             inner, _ptr(log_prob), entropy.data_ptr(), _ptr(top_lp), _ptr(top_id), _ptr(stats), None,
-                             0, temperature, ignore_label is not None, topk, code)
-        with _on_device(dev):
-            ref = ctypes.byref(p)
-            wsb = lib.ldm_label_log_probs_workspace_bytes(ref)
-            if wsb:
-                ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-                p.workspace, p.workspace_bytes = ws.data_ptr(), wsb
-            _check(lib.ldm_label_log_probs(ref, _stream(logits)), "ldm_label_log_probs")
-    return LabelProbs(log_prob, entropy, top_lp, top_id, stats)
+        p = [x.data_ptr(), *n, *s, C, x.stride(dim), y.data_ptr() if y is not None else 0,
+             int(ignore_label) if ignore_label is not None else 0, mask.data_ptr() if mask is not None else 0,
+             mask_stride, mask_div, inner, lp.data_ptr() if lp is not None else 0, entropy.data_ptr(),
+             top_lp.data_ptr() if topk else 0, top_id.data_ptr() if topk else 0,
+             stats.data_ptr() if want_stats else 0, 0, 0, temperature, ignore_label is not None, topk, code]
+        packed = _LABEL_PARAMS.pack(*p)
+        wsb = lib.ldm_label_log_probs_workspace_bytes(packed)
+        if wsb:
+            ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+            p[20], p[21] = ws.data_ptr(), wsb
+            packed = _LABEL_PARAMS.pack(*p)
+        rc = _launch(dev, lib.ldm_label_log_probs, packed)
+        if rc:
+            _check(rc, "ldm_label_log_probs")
+    return LabelProbs(lp, entropy, top_lp, top_id, stats)
 
 
 def _upstream(g, shape, dev, name):
-    if g is None:
-        return None
     if g.dtype != torch.float32 or g.device != dev or g.shape != shape:
         raise ValueError(f"{name} must be fp32 {tuple(shape)} on the logits' device")
     return g.contiguous()
@@ -2022,27 +2039,26 @@ def label_log_probs_bwd(logits, stats, d_log_prob=None, d_entropy=None, *, dim=1
     """The logits' gradient (their shape, type and layout) from the gradients of label_log_probs' log_prob and
     entropy (fp32 [positions], either may be None), its ``stats`` and its other arguments.  Masked classes,
     rows without a class and log_prob of ignored, invalid or impossible labels get none."""
-    code = dtype_code(logits.dtype)
-    dim = _label_dim(logits, dim)
-    temperature = _label_temperature(temperature)
-    pos_shape = logits.shape[:dim] + logits.shape[dim + 1:]
+    dim, pos_shape, code = _label_checked(logits, dim, temperature)
     dev = logits.device
     if stats.dtype != torch.float32 or stats.device != dev or stats.shape != (4,) + pos_shape \
             or not stats.is_contiguous():
         raise ValueError(f"stats must be label_log_probs' fp32 {(4,) + tuple(pos_shape)}")
-    gl = _upstream(d_log_prob, pos_shape, dev, "d_log_prob")
-    ge = _upstream(d_entropy, pos_shape, dev, "d_entropy")
+    gl = None if d_log_prob is None else _upstream(d_log_prob, pos_shape, dev, "d_log_prob")
+    ge = None if d_entropy is None else _upstream(d_entropy, pos_shape, dev, "d_entropy")
     N = math.prod(pos_shape)
-    mask, mask_stride, mask_div = _label_mask(class_mask, logits, dim, N)
+    mask, mask_stride, mask_div = (None, 0, 1) if class_mask is None else _label_mask(class_mask, logits, dim, N)
     _gpu(logits)
-    lib = load_library()
-    x, n, s, _, _, out, o = _label_positions(logits, dim, grad=True)
+    lib = _lib or load_library()
+    x, n, s, _, out, o = _label_positions(logits, dim, torch.empty_like(logits))
     if N:
-        p = LabelProbsBwdParams(x.data_ptr(), *n, *s, x.shape[dim], x.stride(dim), _ptr(mask), mask_stride, mask_div,
-                                stats.data_ptr(), _ptr(gl), _ptr(ge), out.data_ptr(), *o, out.stride(dim), temperature,
-                                code)
-        with _on_device(dev):
-            _check(lib.ldm_label_log_probs_bwd(ctypes.byref(p), _stream(logits)), "ldm_label_log_probs_bwd")
+        packed = _LABEL_BWD_PARAMS.pack(
+            x.data_ptr(), *n, *s, x.shape[dim], x.stride(dim), mask.data_ptr() if mask is not None else 0, mask_stride,
+            mask_div, stats.data_ptr(), gl.data_ptr() if gl is not None else 0, ge.data_ptr() if ge is not None else 0,
+            out.data_ptr(), *o, out.stride(dim), temperature, code)
+        rc = _launch(dev, lib.ldm_label_log_probs_bwd, packed)
+        if rc:
+            _check(rc, "ldm_label_log_probs_bwd")
     return out
 
 
@@ -2054,21 +2070,18 @@ NORM_TYPES = {2.0: 0, math.inf: 1, 1.0: 2}
 
 def _grad_arrays(grads):
     """Host arrays (addresses, element counts, dtype codes) of dense gradients on one GPU, and their device."""
-    dev = grads[0].device
+    T = torch.Tensor
     try:
-        codes = bytes([_GRAD_CODES[g.dtype] for g in grads])
+        codes = bytes(map(_GRAD_CODES.__getitem__, map(_dtype_of, grads)))
     except KeyError as e:
         raise TypeError(f"unsupported gradient dtype {e.args[0]}: float32 or bfloat16") from None
-    for g in grads:
-        if g.device != dev:
-            raise ValueError(f"gradients on {dev} and {g.device}: one device per call")
-        if g.layout != torch.strided:
-            raise TypeError("sparse gradients are not supported")
-        if not g.is_contiguous() and not _is_dense(g):
-            raise ValueError("a gradient is no dense memory (an expanded or strided view): make it contiguous")
-    ptrs = array.array("Q", [g.data_ptr() for g in grads])
-    numel = array.array("q", [g.numel() for g in grads])
-    return ptrs, numel, codes, dev
+    if any(map(_is_sparse, grads)):
+        raise TypeError("sparse gradients are not supported")
+    if len(set(map(T.get_device, grads))) > 1:
+        raise ValueError("gradients on several devices: one device per call")
+    if not all(map(T.is_contiguous, grads)) and not all(g.is_contiguous() or _is_dense(g) for g in grads):
+        raise ValueError("a gradient is no dense memory (an expanded or strided view): make it contiguous")
+    return array.array("Q", map(T.data_ptr, grads)), array.array("q", map(T.numel, grads)), codes
 
 
 def _is_dense(t):
@@ -2082,6 +2095,8 @@ def _is_dense(t):
 
 
 _GRAD_CODES = {torch.float32: F32, torch.bfloat16: BF16}
+_dtype_of = operator.attrgetter("dtype")
+_is_sparse = operator.attrgetter("is_sparse")
 
 
 def _grad_norm(grads, norm_type, max_norm, clip, out=None):
@@ -2089,21 +2104,23 @@ def _grad_norm(grads, norm_type, max_norm, clip, out=None):
         raise ValueError(f"norm_type must be 2, inf or 1, got {norm_type}")
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be a number >= 0, got {max_norm}")
-    ptrs, numel, codes, dev = _grad_arrays(grads)
+    ptrs, numel, codes = _grad_arrays(grads)
     _gpu(grads[0])
-    lib = load_library()
-    n = len(grads)
+    lib = _lib or load_library()
+    dev, n = grads[0].device, len(grads)
     at = numel.buffer_info()[0]
     if out is None:
         out = torch.empty(2, dtype=torch.float32, device=dev)
-    wsb = 0 if clip == 2 else lib.ldm_grad_norm_workspace_bytes(at, n)
-    with _on_device(dev):
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-        rc = lib.ldm_grad_norm(ptrs.buffer_info()[0], at, codes, n, NORM_TYPES[norm_type], float(max_norm), clip,
-                               _ptr(out), _ptr(ws), wsb, _stream(out))
+    wsb, ws = 0, None
+    if clip != 2:
+        wsb = lib.ldm_grad_norm_workspace_bytes(at, n)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    rc = _launch(dev, lib.ldm_grad_norm, ptrs.buffer_info()[0], at, codes, n, NORM_TYPES[norm_type], max_norm, clip,
+                 out.data_ptr(), None if ws is None else ws.data_ptr(), wsb)
     if rc == ERR_OVERLAP:
         raise ValueError("gradients overlap in memory (the same gradient twice, or views of one another)")
-    _check(rc, "ldm_grad_norm")
+    if rc:
+        _check(rc, "ldm_grad_norm")
     return out
 
 
