@@ -9,6 +9,8 @@ from ldmseg.ops import native as K
 from ldmseg.trainers import clip_grad_norm_
 from oracle import label_probs as oracle
 
+ERR_OVERLAP = 4
+
 
 def _refuses(exc, match, *a, **kw):
     with pytest.raises(exc, match=match):
@@ -84,8 +86,8 @@ def test_c_entries_refuse_before_any_launch():
     def norm(ptrs=ptrs, numel=numel, codes=b"\0\0", n=2, kind=0, limit=1.0, clip=1, out=64, ws=64, wsb=wsb):
         return lib.ldm_grad_norm(ptrs, numel, codes, n, kind, limit, clip, out, ws, wsb, None)
 
-    assert norm(ptrs=(u64 * 2)(4096, 4096)) == norm(ptrs=(u64 * 2)(4096, 4156)) == K.ERR_OVERLAP
-    assert "overlap" in lib.ldm_status_string(K.ERR_OVERLAP).decode()
+    assert norm(ptrs=(u64 * 2)(4096, 4096)) == norm(ptrs=(u64 * 2)(4096, 4156)) == ERR_OVERLAP
+    assert "overlap" in lib.ldm_status_string(ERR_OVERLAP).decode()
     for kw in (dict(ptrs=(u64 * 2)(0, 8192)),
                dict(numel=(i64 * 2)(-1, 16)), dict(codes=b"\0\2"), dict(n=0), dict(n=-1), dict(kind=3), dict(kind=-1),
                dict(limit=-1.0), dict(limit=math.nan), dict(clip=3), dict(clip=-1), dict(out=None), dict(ws=None),
@@ -117,13 +119,14 @@ def test_clip_refusals():
             K.grad_norm([bad])
     with pytest.raises(TypeError, match="sparse"):
         K.grad_norm([torch.ones(4).to_sparse()])
-
-
-def test_dense_views():
-    x = torch.zeros(2, 3, 4, 5)
-    assert K._is_dense(x.permute(0, 2, 3, 1)) and K._is_dense(x.transpose(0, 3)) and K._is_dense(torch.zeros(()))
-    assert K._is_dense(torch.zeros(3, 0, 2)) and K._is_dense(x[:1]) and K._is_dense(x[1:, :, :, :])
-    assert not K._is_dense(x[:, :2]) and not K._is_dense(x[..., ::2]) and not K._is_dense(x[:1].expand(2, 3, 4, 5))
+    with pytest.raises(TypeError, match="must be a tensor"):
+        K.grad_norm([torch.ones(4), 3])
+    with pytest.raises(TypeError, match="iterable"):
+        K.grad_norm(7)
+    for dense in (torch.zeros(2, 3, 4, 5).permute(0, 2, 3, 1), torch.zeros(3, 0, 2), torch.zeros(()),
+                  torch.zeros(5, 1).expand(5, 1)):
+        with pytest.raises(RuntimeError, match="GPU tensors only"):      # dense in any order: only the device is wrong
+            K.grad_norm([dense])
 
 
 @pytest.mark.parametrize("make,dim", [
@@ -137,7 +140,7 @@ def test_strided_positions_address_every_element(make, dim):
     base = torch.arange(2 * 5 * 6 * 8).view(2, 5, 6, 8)
     x = make(base)
     dim = dim % x.ndim
-    y, n, s, inner, out, o = K._label_positions(x, dim, torch.empty_like(x))
+    y, n, s, inner, out, o = K.torch_binding().label_positions(x, dim)
     N = n[0] * n[1] * n[2]
     idx = [torch.arange(k) for k in n]
     grid = sum(i.view([-1 if j == d else 1 for j in range(3)]) * st for d, (i, st) in enumerate(zip(idx, s)))

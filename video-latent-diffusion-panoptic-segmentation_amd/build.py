@@ -1,4 +1,4 @@
-"""Build the gfx950 HIP library (lib/libldmseg_hip.so) in-tree.
+"""Build the gfx950 HIP library (lib/libldmseg_hip.so) and its torch binding (lib/ldmseg_torch.so) in-tree.
 
     python video-latent-diffusion-panoptic-segmentation_amd/build.py [--force] [--jobs N]
 
@@ -19,6 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "build")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libldmseg_hip.so")
+BINDING = os.path.join(LIB_DIR, "ldmseg_torch.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function",
@@ -47,9 +48,33 @@ def _compile(src, obj):
     return obj
 
 
+def build_binding(force=False, verbose=True):
+    """The C++ torch binding (csrc/torch_binding.cpp): host code, linked against torch's own libraries."""
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    if not force and not _stale(BINDING, [src, *_headers(), os.path.abspath(__file__)]):
+        return BINDING
+    import sysconfig
+
+    import torch
+    if verbose:
+        print("[build] compiling the torch binding", flush=True)
+    inc, lib = (os.path.join(os.path.dirname(torch.__file__), d) for d in ("include", "lib"))
+    rocm = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DUSE_ROCM",
+           "-D__HIP_PLATFORM_AMD__", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + inc,
+           "-I" + sysconfig.get_paths()["include"], "-I" + rocm, src, "-o", BINDING + ".tmp", "-L" + lib, "-lc10",
+           "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"torch binding failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(BINDING + ".tmp", BINDING)
+    return BINDING
+
+
 def build(force=False, jobs=None, verbose=True):
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
+    build_binding(force, verbose)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     hdrs = _headers()
     objs, todo = [], []

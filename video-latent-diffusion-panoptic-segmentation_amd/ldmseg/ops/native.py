@@ -5,14 +5,12 @@ no fallback: if the library is missing, or a tensor is not on the GPU, the call 
 Host-side checks (device, dtype, contiguity, shapes) run before any launch so that a bad
 call can never reach the GPU as an out-of-bounds kernel.
 """
-import array
 import collections
 import contextlib
 import ctypes
+import importlib.util
 import math
-import operator
 import os
-import struct
 import threading
 
 import torch
@@ -21,7 +19,6 @@ PKG_ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__fil
 LIB_PATH = os.path.join(PKG_ROOT, "lib", "libldmseg_hip.so")
 
 F32, BF16 = 0, 1
-ERR_OVERLAP = 4
 OUT_NHWC, OUT_NCHW, OUT_GEGLU, OUT_SHUFFLE2 = 0, 1, 2, 3
 ACT_NONE, ACT_SILU, ACT_RELU, ACT_SIGMOID = 0, 1, 2, 3
 PRED = {"epsilon": 0, "sample": 1, "v_prediction": 2}
@@ -195,9 +192,9 @@ EXPORTS = {
     "ldm_space_to_depth2": (_i, [_vp, _i, _i, _i, _i, _vp, _i, _vp]),
     "ldm_posterior_sample": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp]),
     "ldm_posterior_bwd": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
-    "ldm_label_log_probs_workspace_bytes": (ctypes.c_size_t, [_vp]),
-    "ldm_label_log_probs": (_i, [_vp, _vp]),
-    "ldm_label_log_probs_bwd": (_i, [_vp, _vp]),
+    "ldm_label_log_probs_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LabelProbsParams)]),
+    "ldm_label_log_probs": (_i, [ctypes.POINTER(LabelProbsParams), _vp]),
+    "ldm_label_log_probs_bwd": (_i, [ctypes.POINTER(LabelProbsBwdParams), _vp]),
     "ldm_grad_norm_workspace_bytes": (ctypes.c_size_t, [_vp, _i]),
     "ldm_grad_norm": (_i, [_vp, _vp, _vp, _i, _i, _d, _i, _vp, _vp, _i64, _vp]),
     "ldm_status_string": (ctypes.c_char_p, [_i]),
@@ -261,17 +258,29 @@ def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
-    lambda i: torch.cuda.current_stream(i).cuda_stream
+_torch = None
 
 
-def _launch(dev, fn, *args):
-    """fn(*args, stream) with ``dev`` as the current device, on its current stream."""
-    i = dev.index
-    if i == torch.cuda.current_device():
-        return fn(*args, _raw_stream(i))
-    with torch.cuda.device(i):
-        return fn(*args, _raw_stream(i))
+def torch_binding():
+    """The C++ binding of the operators that are called often or with long lists of tensors (csrc/torch_binding.cpp,
+    lib/ldmseg_torch.so), bound to the loaded HIP library."""
+    global _torch
+    lib = load_library()
+    with _lock:
+        if _torch is None:
+            path = os.path.join(PKG_ROOT, "lib", "ldmseg_torch.so")
+            if not os.path.exists(path):
+                raise RuntimeError(f"ldmseg torch binding not found at {path}: run "
+                                   f"`python video-latent-diffusion-panoptic-segmentation_amd/build.py` "
+                                   f"(or __graft_entry__.build()) first")
+            spec = importlib.util.spec_from_file_location("ldmseg_torch", path)
+            m = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(m)
+            m.init(*(ctypes.cast(f, _vp).value for f in (
+                lib.ldm_label_log_probs_workspace_bytes, lib.ldm_label_log_probs, lib.ldm_label_log_probs_bwd,
+                lib.ldm_grad_norm_workspace_bytes, lib.ldm_grad_norm, lib.ldm_status_string)))
+            _torch = m
+    return _torch
 
 
 def _contig(t, name):
@@ -1883,92 +1892,6 @@ def posterior_bwd(moments, eps, dz_nhwc):
 LABEL_TOPK_MAX = 16
 LabelProbs = collections.namedtuple("LabelProbs", "log_prob entropy top_log_probs top_ids stats")
 
-# LabelProbsParams / LabelProbsBwdParams as bytes (a ctypes.Structure takes several times as long to fill)
-_LABEL_PARAMS = struct.Struct("@22qf3i")
-_LABEL_BWD_PARAMS = struct.Struct("@20qfi")
-assert _LABEL_PARAMS.size == ctypes.sizeof(LabelProbsParams)
-assert _LABEL_BWD_PARAMS.size == ctypes.sizeof(LabelProbsBwdParams)
-
-
-def _merge_dims(sizes, *strides):
-    """(sizes, strides...) without dims of size 1 and with adjacent dims merged where every layout has them
-    one stride apart."""
-    ns, out = [], [[] for _ in strides]
-    for i, n in enumerate(sizes):
-        if n == 1:
-            continue
-        if ns and all(o[-1] == n * s[i] for o, s in zip(out, strides)):
-            ns[-1] *= n
-            for o, s in zip(out, strides):
-                o[-1] = s[i]
-        else:
-            ns.append(n)
-            for o, s in zip(out, strides):
-                o.append(s[i])
-    return ns, out
-
-
-def _label_positions(x, dim, out=None):
-    """The positions of ``x`` (every dim but ``dim``) as three strided dims: (x, sizes, strides, positions behind
-    the class dim, out, out's strides).  Dims are merged on either side of the class dim, never across it; a tensor
-    with more than three left is copied.  ``out``: a tensor like x that is walked by the same sizes."""
-    shape = x.shape
-    if x.is_contiguous():
-        inner = math.prod(shape[dim + 1:])
-        s = (0, shape[dim] * inner, 1)
-        return x, (1, math.prod(shape[:dim]), inner), s, inner, out, s
-    st = x.stride()
-    if dim == 1:
-        so = st if out is None else out.stride()
-        if x.ndim == 4 and 1 not in shape:
-            n, h, w = shape[0], shape[2], shape[3]
-            if st[2] == w * st[3] and so[2] == w * so[3]:
-                return x, (1, n, h * w), (0, st[0], st[3]), h * w, out, (0, so[0], so[3])
-            return x, (n, h, w), (st[0], st[2], st[3]), h * w, out, (so[0], so[2], so[3])
-        if x.ndim == 2:
-            return x, (1, 1, shape[0]), (0, 0, st[0]), 1, out, (0, 0, so[0])
-    layouts = [st] if out is None else [st, out.stride()]
-    no, so = _merge_dims(shape[:dim], *[t[:dim] for t in layouts])
-    ni, si = _merge_dims(shape[dim + 1:], *[t[dim + 1:] for t in layouts])
-    n = no + ni
-    if len(n) > 3:
-        x = x.contiguous()
-        return _label_positions(x, dim, None if out is None else torch.empty_like(x))
-    pad = 3 - len(n)
-    s = [[0] * pad + a + b for a, b in zip(so, si)]
-    return x, [1] * pad + n, s[0], math.prod(ni), out, s[-1]
-
-
-def _label_mask(class_mask, logits, dim, n_positions):
-    """(mask, row stride, positions to a row) of a class mask [C] or [logits.shape[0], C]."""
-    C, B = logits.shape[dim], logits.shape[0]
-    if class_mask.dtype != torch.bool or class_mask.device != logits.device:
-        raise TypeError("class_mask must be a bool tensor on the logits' device")
-    if tuple(class_mask.shape) == (C,):
-        return class_mask.contiguous(), 0, max(1, n_positions)
-    if dim != 0 and tuple(class_mask.shape) == (B, C):
-        return class_mask.contiguous(), C, max(1, n_positions // max(1, B))
-    raise ValueError(f"class_mask must be [{C}] or [{B}, {C}] (classes, or the logits' first dim by classes), got "
-                     f"{tuple(class_mask.shape)}")
-
-
-def _label_checked(logits, dim, temperature):
-    """(class dim, positions' shape, dtype code) of checked arguments."""
-    code = dtype_code(logits.dtype)
-    nd = logits.ndim
-    if nd < 2:
-        raise ValueError("logits need a class dim and at least one position dim")
-    if not -nd <= dim < nd:
-        raise ValueError(f"class dim {dim} is outside logits of {nd} dims")
-    dim %= nd
-    shape = logits.shape
-    if shape[dim] == 0:
-        raise ValueError("logits have no classes")
-    if not 1e-4 <= temperature <= 1e4:
-        raise ValueError(f"temperature must be in [1e-4, 1e4], got {temperature}")
-    return dim, shape[:dim] + shape[dim + 1:], code
-
-
 def label_log_probs(logits, labels=None, *, dim=1, topk=0, temperature=1.0, ignore_label=None, class_mask=None,
                     want_stats=False):
     """Per position of ``logits`` (fp32 / bf16, any strides, classes along ``dim``), in one pass over them,
@@ -1986,80 +1909,16 @@ def label_log_probs(logits, labels=None, *, dim=1, topk=0, temperature=1.0, igno
     ``class_mask`` (bool [C] or [logits.shape[0], C]) leaves classes out whatever their logits hold.  A row
     that is left without a class has entropy 0 and no alternatives; a NaN or +inf among the classes left
     makes the row's log_prob and entropy NaN."""
-    dim, pos_shape, code = _label_checked(logits, dim, temperature)
-    C = logits.shape[dim]
-    if not 0 <= topk <= min(C, LABEL_TOPK_MAX):
-        raise ValueError(f"topk must be in [0, {min(C, LABEL_TOPK_MAX)}], got {topk}")
-    dev = logits.device
-    y = lp = top_lp = top_id = stats = None
-    if labels is not None:
-        if labels.dtype != torch.int64 or labels.device != dev:
-            raise TypeError("labels must be an int64 tensor on the logits' device")
-        if labels.shape != pos_shape:
-            raise ValueError(f"labels must be {tuple(pos_shape)}, got {tuple(labels.shape)}")
-        y = labels.contiguous()
-    N = math.prod(pos_shape)
-    mask, mask_stride, mask_div = (None, 0, 1) if class_mask is None else _label_mask(class_mask, logits, dim, N)
-    _gpu(logits)
-    lib = _lib or load_library()
-    x, n, s, inner, _, _ = _label_positions(logits, dim)
-    entropy = torch.empty(pos_shape, dtype=torch.float32, device=dev)
-    if y is not None:
-        lp = torch.empty_like(entropy)
-    if topk:
-        top_lp = entropy.new_empty(logits.shape[:dim] + (topk,) + logits.shape[dim + 1:])
-        top_id = torch.empty_like(top_lp, dtype=torch.int32)
-    if want_stats:
-        stats = entropy.new_empty((4,) + pos_shape)
-    if N:
-        p = [x.data_ptr(), *n, *s, C, x.stride(dim), y.data_ptr() if y is not None else 0,
-             int(ignore_label) if ignore_label is not None else 0, mask.data_ptr() if mask is not None else 0,
-             mask_stride, mask_div, inner, lp.data_ptr() if lp is not None else 0, entropy.data_ptr(),
-             top_lp.data_ptr() if topk else 0, top_id.data_ptr() if topk else 0,
-             stats.data_ptr() if want_stats else 0, 0, 0, temperature, ignore_label is not None, topk, code]
-        packed = _LABEL_PARAMS.pack(*p)
-        wsb = lib.ldm_label_log_probs_workspace_bytes(packed)
-        if wsb:
-            ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-            p[20], p[21] = ws.data_ptr(), wsb
-            packed = _LABEL_PARAMS.pack(*p)
-        rc = _launch(dev, lib.ldm_label_log_probs, packed)
-        if rc:
-            _check(rc, "ldm_label_log_probs")
-    return LabelProbs(lp, entropy, top_lp, top_id, stats)
-
-
-def _upstream(g, shape, dev, name):
-    if g.dtype != torch.float32 or g.device != dev or g.shape != shape:
-        raise ValueError(f"{name} must be fp32 {tuple(shape)} on the logits' device")
-    return g.contiguous()
+    return LabelProbs(*(_torch or torch_binding()).label_log_probs(logits, labels, dim, topk, temperature, ignore_label,
+                                                                   class_mask, want_stats))
 
 
 def label_log_probs_bwd(logits, stats, d_log_prob=None, d_entropy=None, *, dim=1, temperature=1.0, class_mask=None):
     """The logits' gradient (their shape, type and layout) from the gradients of label_log_probs' log_prob and
     entropy (fp32 [positions], either may be None), its ``stats`` and its other arguments.  Masked classes,
     rows without a class and log_prob of ignored, invalid or impossible labels get none."""
-    dim, pos_shape, code = _label_checked(logits, dim, temperature)
-    dev = logits.device
-    if stats.dtype != torch.float32 or stats.device != dev or stats.shape != (4,) + pos_shape \
-            or not stats.is_contiguous():
-        raise ValueError(f"stats must be label_log_probs' fp32 {(4,) + tuple(pos_shape)}")
-    gl = None if d_log_prob is None else _upstream(d_log_prob, pos_shape, dev, "d_log_prob")
-    ge = None if d_entropy is None else _upstream(d_entropy, pos_shape, dev, "d_entropy")
-    N = math.prod(pos_shape)
-    mask, mask_stride, mask_div = (None, 0, 1) if class_mask is None else _label_mask(class_mask, logits, dim, N)
-    _gpu(logits)
-    lib = _lib or load_library()
-    x, n, s, _, out, o = _label_positions(logits, dim, torch.empty_like(logits))
-    if N:
-        packed = _LABEL_BWD_PARAMS.pack(
-            x.data_ptr(), *n, *s, x.shape[dim], x.stride(dim), mask.data_ptr() if mask is not None else 0, mask_stride,
-            mask_div, stats.data_ptr(), gl.data_ptr() if gl is not None else 0, ge.data_ptr() if ge is not None else 0,
-            out.data_ptr(), *o, out.stride(dim), temperature, code)
-        rc = _launch(dev, lib.ldm_label_log_probs_bwd, packed)
-        if rc:
-            _check(rc, "ldm_label_log_probs_bwd")
-    return out
+    return (_torch or torch_binding()).label_log_probs_bwd(logits, stats, d_log_prob, d_entropy, dim, temperature,
+                                                           class_mask)
 
 
 # ======================================================================================
@@ -2068,69 +1927,24 @@ def label_log_probs_bwd(logits, stats, d_log_prob=None, d_entropy=None, *, dim=1
 NORM_TYPES = {2.0: 0, math.inf: 1, 1.0: 2}
 
 
-def _grad_arrays(grads):
-    """Host arrays (addresses, element counts, dtype codes) of dense gradients on one GPU, and their device."""
-    T = torch.Tensor
-    try:
-        codes = bytes(map(_GRAD_CODES.__getitem__, map(_dtype_of, grads)))
-    except KeyError as e:
-        raise TypeError(f"unsupported gradient dtype {e.args[0]}: float32 or bfloat16") from None
-    if any(map(_is_sparse, grads)):
-        raise TypeError("sparse gradients are not supported")
-    if len(set(map(T.get_device, grads))) > 1:
-        raise ValueError("gradients on several devices: one device per call")
-    if not all(map(T.is_contiguous, grads)) and not all(g.is_contiguous() or _is_dense(g) for g in grads):
-        raise ValueError("a gradient is no dense memory (an expanded or strided view): make it contiguous")
-    return array.array("Q", map(T.data_ptr, grads)), array.array("q", map(T.numel, grads)), codes
-
-
-def _is_dense(t):
-    """Whether a tensor's elements are one gapless span of memory, in any order of its dims."""
-    need = 1
-    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if st != need:
-            return t.numel() == 0
-        need *= n
-    return True
-
-
-_GRAD_CODES = {torch.float32: F32, torch.bfloat16: BF16}
-_dtype_of = operator.attrgetter("dtype")
-_is_sparse = operator.attrgetter("is_sparse")
-
-
-def _grad_norm(grads, norm_type, max_norm, clip, out=None):
-    if norm_type not in NORM_TYPES:
+def _grad_norm(tensors, of_params, norm_type, max_norm, clip, out=None):
+    """(norm, [norm, factor]) of tensors, or of their gradients; None where there are none.  ``clip`` as in
+    ldm_grad_norm."""
+    kind = NORM_TYPES.get(norm_type)
+    if kind is None:
         raise ValueError(f"norm_type must be 2, inf or 1, got {norm_type}")
-    if not max_norm >= 0:
-        raise ValueError(f"max_norm must be a number >= 0, got {max_norm}")
-    ptrs, numel, codes = _grad_arrays(grads)
-    _gpu(grads[0])
-    lib = _lib or load_library()
-    dev, n = grads[0].device, len(grads)
-    at = numel.buffer_info()[0]
-    if out is None:
-        out = torch.empty(2, dtype=torch.float32, device=dev)
-    wsb, ws = 0, None
-    if clip != 2:
-        wsb = lib.ldm_grad_norm_workspace_bytes(at, n)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    rc = _launch(dev, lib.ldm_grad_norm, ptrs.buffer_info()[0], at, codes, n, NORM_TYPES[norm_type], max_norm, clip,
-                 out.data_ptr(), None if ws is None else ws.data_ptr(), wsb)
-    if rc == ERR_OVERLAP:
-        raise ValueError("gradients overlap in memory (the same gradient twice, or views of one another)")
-    if rc:
-        _check(rc, "ldm_grad_norm")
-    return out
+    return (_torch or torch_binding()).grad_norm(tensors, of_params, kind, max_norm, clip, out)
 
 
 def grad_norm(grads, norm_type=2.0):
     """Global norm (2, inf or 1) of a list of dense fp32 / bf16 gradients on one GPU, any mix of types and
     sizes -> 0-d fp32 device tensor; fp64 sums, no host synchronisation."""
-    return _grad_norm(grads, norm_type, 0.0, 0)[0]
+    r = _grad_norm(grads, False, norm_type, 0.0, 0)
+    return torch.tensor(0.0) if r is None else r[0]
 
 
 def clip_grads(grads, max_norm, norm_type=2.0):
     """grad_norm, then every gradient times min(1, max_norm / (norm + 1e-6)) in place (nothing is written
     where the factor is 1) -> the norm before clipping.  Gradients must not overlap."""
-    return _grad_norm(grads, norm_type, max_norm, 1)[0]
+    r = _grad_norm(grads, False, norm_type, max_norm, 1)
+    return torch.tensor(0.0) if r is None else r[0]

@@ -16,16 +16,17 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     factor as torch does (inf: 0, NaN: NaN) unless ``error_if_nonfinite``, which raises before anything is
     scaled and is the only form that waits for the GPU.  A gradient listed twice is refused."""
     if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
-    grads = [g for p in parameters if (g := p.grad) is not None]
-    if not grads:
-        return torch.tensor(0.0)
+        parameters = (parameters,)
     norm_type = float(norm_type)
     if not error_if_nonfinite:
-        return K.clip_grads(grads, max_norm, norm_type)
-    out = K._grad_norm(grads, norm_type, max_norm, 0)
-    if not torch.isfinite(out[0]):
+        r = K._grad_norm(parameters, True, norm_type, max_norm, 1)
+        return torch.tensor(0.0) if r is None else r[0]
+    parameters = list(parameters)
+    r = K._grad_norm(parameters, True, norm_type, max_norm, 0)
+    if r is None:
+        return torch.tensor(0.0)
+    if not torch.isfinite(r[0]):
         raise RuntimeError(f"the gradients' norm of order {norm_type} is not finite, so they cannot be clipped; "
                            "error_if_nonfinite=False scales them all the same")
-    K._grad_norm(grads, norm_type, max_norm, 2, out)
-    return out[0]
+    K._grad_norm(parameters, True, norm_type, max_norm, 2, r[1])
+    return r[0]
