@@ -777,7 +777,7 @@ int ldm_label_log_probs_bwd(const ldm_label_probs_bwd_params* p, ldm_stream_t st
  *   clip                  0: norm only.  1: norm, then every g *= factor where the factor is below
  *                         1 or NaN (torch.nn.utils.clip_grad_norm_'s arithmetic).  2: only the
  *                         scaling, by the factor already in out
- * Sums run in a fixed order (no atomics): the same gradients give the same bits. */
+ * Sums run in an order that the addresses fix (no atomics): the same call gives the same bits. */
 enum { LDM_NORM_2 = 0, LDM_NORM_INF = 1, LDM_NORM_1 = 2 };
 size_t ldm_grad_norm_workspace_bytes(const int64_t* numel, int ntensors);
 int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, const uint8_t* dtypes, int ntensors, int norm_type,

@@ -2,8 +2,9 @@
 //
 //   norm   = sqrt(sum g^2), max |g| or sum |g| over every element of every tensor
 //   factor = min(1, max_norm / (norm + 1e-6));  g *= factor   (torch.nn.utils.clip_grad_norm_)
-// The spans' addresses travel as kernel arguments, up to TABLE of them to a launch: nothing is
-// copied to the device, nothing is kept between calls, and a captured graph holds its own table.
+// The spans' addresses travel as kernel arguments, up to TABLE of them to a launch; more are listed
+// in the workspace by a launch for each table.  Nothing is copied from the host, nothing is kept
+// between calls, and a captured graph holds its own tables.
 // Squares are summed in fp64 (a square of any fp32 value is finite there), per thread, block and
 // partial in a fixed order: the same gradients give the same bits.
 #include "common.h"
@@ -50,33 +51,41 @@ template <int NORM> __device__ __forceinline__ double norm_join(double a, double
   if (NORM != LDM_NORM_INF) return a + b;
   return (b > a || b != b) ? b : a;
 }
-template <int NORM> __device__ __forceinline__ double block_join(double v) {
-  __shared__ double part[4];
+template <int NORM, int WAVES = 4> __device__ __forceinline__ double block_join(double v) {
+  __shared__ double part[WAVES];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = norm_join<NORM>(v, __shfl_xor(v, o, 64));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
-  return norm_join<NORM>(norm_join<NORM>(part[0], part[1]), norm_join<NORM>(part[2], part[3]));
+  v = part[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) v = norm_join<NORM>(v, part[w]);
+  return v;
 }
 
-// A thread's packs of a chunk's elements [0, n), at any address aligned to one element: all loads in flight.
-// pack(index, pack) for each whole one, rest(element) for the elements behind the last.
-template <typename T, typename P, typename R>
-__device__ __forceinline__ void each_pack(const T* g, int n, P pack, R rest) {
+// A thread's packs of a chunk's elements [0, n), at any address aligned to one element: all loads in flight, then
+// ready() (false: nothing more), pack(index, pack) for each whole one and rest(element, value) for an element behind
+// the last.
+template <typename T, typename Q, typename P, typename R>
+__device__ __forceinline__ void each_pack(const T* g, int n, Q ready, P pack, R rest) {
   constexpr int V = 16 / (int)sizeof(T);
   Pack<T> p[PACKS];
   if (n == chunk_of<T>()) {
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) __builtin_memcpy(&p[i], g + (i * 256 + threadIdx.x) * V, 16);
+    if (!ready()) return;
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) pack(i * 256 + (int)threadIdx.x, p[i]);
     return;
   }
   const int whole = n / V, last = whole * V + (int)threadIdx.x;
+  T tail = T(0);
+  if (last < n) tail = g[last];
 #pragma unroll
   for (int i = 0; i < PACKS; ++i)
     if (i * 256 + (int)threadIdx.x < whole) __builtin_memcpy(&p[i], g + (i * 256 + threadIdx.x) * V, 16);
-  if (last < n) rest(last);
+  if (!ready()) return;
+  if (last < n) rest(last, tail);
 #pragma unroll
   for (int i = 0; i < PACKS; ++i)
     if (i * 256 + (int)threadIdx.x < whole) pack(i * 256 + (int)threadIdx.x, p[i]);
@@ -84,28 +93,47 @@ __device__ __forceinline__ void each_pack(const T* g, int n, P pack, R rest) {
 
 template <int NORM, typename T>
 __device__ __forceinline__ double chunk_norm(const T* g, int n, double acc) {
-  each_pack(g, n, [&](int, const Pack<T>& p) {
+  each_pack(g, n, [] { return true; }, [&](int, const Pack<T>& p) {
 #pragma unroll
     for (int j = 0; j < 16 / (int)sizeof(T); ++j) acc = norm_add<NORM>(acc, to_f(p.v[j]));
-  }, [&](int i) { acc = norm_add<NORM>(acc, to_f(g[i])); });
+  }, [&](int, T v) { acc = norm_add<NORM>(acc, to_f(v)); });
   return acc;
 }
 
-// chunk c of a table: calls f(pointer, elements) with the span's type
-template <typename F> __device__ __forceinline__ void with_chunk(const Table& t, int c, F f) {
+// Where a kernel's chunks come from: a table in its arguments, or (more spans than a table holds) a list in the
+// workspace that list_chunks wrote.  with_chunk calls f(pointer, elements) with chunk c's type.
+struct Chunk {
+  uint64_t ptr;                          // bit 63: bf16
+  int n;
+};
+struct ChunkList {
+  const Chunk* at;
+  int chunks;
+};
+__device__ __forceinline__ Chunk chunk_at(const ChunkList& l, int c) { return l.at[c]; }
+__device__ __forceinline__ Chunk chunk_of_entry(const Entry& e, int k) {
+  const int64_t len = e.ptr >> 63 ? chunk_of<bf16_t>() : chunk_of<float>(), at = k * len;
+  return {e.ptr + (uint64_t)k * (256 * PACKS * 16), (int)min(len, (int64_t)e.n - at)};
+}
+__device__ __forceinline__ Chunk chunk_at(const Table& t, int c) {
   const Entry e = t.e[entry_of(t, c)];
-  const int64_t k = c - (int)e.chunk0;
-  if (e.ptr >> 63) {
-    const int64_t at = k * chunk_of<bf16_t>();
-    f((bf16_t*)(e.ptr & ~(1ull << 63)) + at, (int)min((int64_t)chunk_of<bf16_t>(), (int64_t)e.n - at));
-  } else {
-    const int64_t at = k * chunk_of<float>();
-    f((float*)e.ptr + at, (int)min((int64_t)chunk_of<float>(), (int64_t)e.n - at));
-  }
+  return chunk_of_entry(e, c - (int)e.chunk0);
+}
+template <typename S, typename F> __device__ __forceinline__ void with_chunk(const S& s, int c, F f) {
+  const Chunk k = chunk_at(s, c);
+  if (k.ptr >> 63) f((bf16_t*)(k.ptr & ~(1ull << 63)), k.n);
+  else f((float*)k.ptr, k.n);
 }
 
-template <int NORM>
-__global__ __launch_bounds__(256) void norm_parts(const Table t, double* __restrict__ part) {
+// a table's chunks, a block for each span
+__global__ __launch_bounds__(64) void list_chunks(const Table t, Chunk* __restrict__ to) {
+  const Entry e = t.e[blockIdx.x];
+  const int n = (blockIdx.x + 1 < (unsigned)t.count ? (int)t.e[blockIdx.x + 1].chunk0 : t.chunks) - (int)e.chunk0;
+  for (int k = threadIdx.x; k < n; k += 64) to[(int)e.chunk0 + k] = chunk_of_entry(e, k);
+}
+
+template <int NORM, typename S>
+__global__ __launch_bounds__(256) void norm_parts(const S t, double* __restrict__ part) {
   double acc = 0.0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x)
     with_chunk(t, c, [&](const auto* g, int n) { acc = chunk_norm<NORM>(g, n, acc); });
@@ -138,34 +166,117 @@ __global__ __launch_bounds__(256) void norm_final(const double* __restrict__ par
 
 // a gradient is multiplied by the factor as its own type holds it and rounded once, as torch's in-place product
 // of a tensor with a device scalar is: a bf16 gradient's factor has 8 bits
-template <typename T>
-__device__ __forceinline__ void chunk_scale(T* g, int n, float factor) {
+template <typename T, typename F>
+__device__ __forceinline__ void chunk_scale(T* g, int n, F factor) {
   constexpr int V = 16 / (int)sizeof(T);
-  const float f = to_f(from_f<T>(factor));
-  if (f == 1.f) return;
-  each_pack(g, n, [&](int i, Pack<T> p) {
+  float f;
+  each_pack(g, n, [&] { f = to_f(from_f<T>(factor())); return f != 1.f; }, [&](int i, Pack<T> p) {
 #pragma unroll
     for (int j = 0; j < V; ++j) p.v[j] = from_f<T>(to_f(p.v[j]) * f);
     __builtin_memcpy(g + i * V, &p, 16);
-  }, [&](int i) { g[i] = from_f<T>(to_f(g[i]) * f); });
+  }, [&](int i, T v) { g[i] = from_f<T>(to_f(v) * f); });
 }
 
 // the last chunks first: the norm's pass has left them in the memory-side cache
-__device__ __forceinline__ void scale_chunks(const Table& t, float f) {
+template <typename S>
+__global__ __launch_bounds__(256) void scale_all(const S t, const float* __restrict__ out) {
+  const float f = out[1];
   if (f == 1.f) return;
   for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x)
-    with_chunk(t, c, [&](auto* g, int n) { chunk_scale(g, n, f); });
+    with_chunk(t, c, [&](auto* g, int n) { chunk_scale(g, n, [&] { return f; }); });
 }
-__global__ __launch_bounds__(256) void scale_all(const Table t, const float* __restrict__ out) {
-  scale_chunks(t, out[1]);
-}
-// the same for one table with few partials: every block joins them itself, which takes a launch less
-template <int NORM>
-__global__ __launch_bounds__(256) void scale_joined(const Table t, const double* __restrict__ part, int parts,
+// the same where partials are few: every block joins them itself, beside its first chunk's loads, which takes a
+// launch less
+template <int NORM, typename S>
+__global__ __launch_bounds__(256) void scale_joined(const S t, const double* __restrict__ part, int parts,
                                                     float max_norm, float* __restrict__ out) {
-  const float2 r = norm_of<NORM>(part, parts, max_norm);
-  if (blockIdx.x == 0 && threadIdx.x == 0) { out[0] = r.x; out[1] = r.y; }
-  scale_chunks(t, r.y);
+  float f = -1.f;
+  for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0 && f != 1.f; c -= gridDim.x)
+    with_chunk(t, c, [&](auto* g, int n) {
+      chunk_scale(g, n, [&] {
+        if (f == -1.f) {
+          const float2 r = norm_of<NORM>(part, parts, max_norm);
+          if (blockIdx.x == 0 && threadIdx.x == 0) { out[0] = r.x; out[1] = r.y; }
+          f = r.y;
+        }
+        return f;
+      });
+    });
+}
+
+// Few gradients in one launch of one block: every thread holds up to UNITS packs between the norm and the product,
+// so nothing is read twice.  A unit is a wave's 64 packs of one span; `span` names each unit's.
+constexpr int UNITS = 5, SMALL_WAVES = 16, SMALL_SPANS = 208;
+struct SmallTable {
+  Entry e[SMALL_SPANS];                    // chunk0: the span's first unit
+  uint8_t span[UNITS * SMALL_WAVES];
+  int units;
+};
+template <typename T> __device__ __forceinline__ uint4 load_part(const T* g, int n) {   // n elements, then zeros
+  constexpr int V = 16 / (int)sizeof(T);
+  Pack<T> p;
+  if (n >= V) {
+    __builtin_memcpy(&p, g, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) p.v[j] = j < n ? g[j] : T(0);
+  }
+  return __builtin_bit_cast(uint4, p);
+}
+template <int NORM, typename T> __device__ __forceinline__ double part_norm(const uint4& r, double acc) {
+  const Pack<T> p = __builtin_bit_cast(Pack<T>, r);
+#pragma unroll
+  for (int j = 0; j < 16 / (int)sizeof(T); ++j) acc = norm_add<NORM>(acc, to_f(p.v[j]));
+  return acc;
+}
+template <typename T> __device__ __forceinline__ void store_part(T* g, int n, const uint4& r, float f) {
+  constexpr int V = 16 / (int)sizeof(T);
+  Pack<T> p = __builtin_bit_cast(Pack<T>, r);
+#pragma unroll
+  for (int j = 0; j < V; ++j) p.v[j] = from_f<T>(to_f(p.v[j]) * f);
+  if (n >= V) {
+    __builtin_memcpy(g, &p, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < n) g[j] = p.v[j];
+  }
+}
+template <int NORM>
+__global__ __launch_bounds__(64 * SMALL_WAVES) void clip_small(const SmallTable t, float max_norm, int clip,
+                                                               float* __restrict__ out) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  uint4 r[UNITS];
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const int u = i * SMALL_WAVES + wave;
+    if (u < t.units) {
+      const Entry e = t.e[t.span[u]];
+      const int pack = (u - (int)e.chunk0) * 64 + lane, n = (int)e.n;
+      r[i] = e.ptr >> 63 ? load_part((const bf16_t*)(e.ptr & ~(1ull << 63)) + min(pack * 8, n), n - pack * 8)
+                         : load_part((const float*)e.ptr + min(pack * 4, n), n - pack * 4);
+    }
+  }
+  double acc = 0.0;
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const int u = i * SMALL_WAVES + wave;
+    if (u < t.units) acc = t.e[t.span[u]].ptr >> 63 ? part_norm<NORM, bf16_t>(r[i], acc) : part_norm<NORM, float>(r[i], acc);
+  }
+  acc = block_join<NORM, SMALL_WAVES>(acc);
+  const float norm = (float)(NORM == LDM_NORM_2 ? sqrt(acc) : acc), f = factor_of(norm, max_norm);
+  if (threadIdx.x == 0) { out[0] = norm; out[1] = f; }
+  if (!clip || f == 1.f) return;
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const int u = i * SMALL_WAVES + wave;
+    if (u < t.units) {
+      const Entry e = t.e[t.span[u]];
+      const int pack = (u - (int)e.chunk0) * 64 + lane, n = (int)e.n;
+      if (e.ptr >> 63) store_part((bf16_t*)(e.ptr & ~(1ull << 63)) + min(pack * 8, n), n - pack * 8, r[i], to_f(from_f<bf16_t>(f)));
+      else store_part((float*)e.ptr + min(pack * 4, n), n - pack * 4, r[i], f);
+    }
+  }
 }
 
 // a span above 2^30 elements is listed in pieces (of whole chunks)
@@ -176,40 +287,54 @@ int64_t entries_of(const int64_t* numel, int n) {
   return c;
 }
 
-constexpr int JOIN_PARTS = 512;          // two partials a thread
+constexpr int JOIN_CHUNKS = 1024;        // a pass of few chunks: a launch costs more than every block's own join
 
-template <int NORM>
-int launch(const std::vector<Table>& tables, float max_norm, int clip, float* out, double* part, hipStream_t s) {
-  int parts = 0;
+template <int NORM, typename S>
+int launch(const S& t, float max_norm, int clip, float* out, double* part, hipStream_t s) {
+  const dim3 grid(std::max(1, std::min(t.chunks, MAX_BLOCKS))), block(256);
   if (clip != 2) {
-    for (const Table& t : tables) {
-      const int blocks = std::min(t.chunks, MAX_BLOCKS);
-      hipLaunchKernelGGL((norm_parts<NORM>), dim3(blocks), dim3(256), 0, s, t, part + parts);
-      LDM_CHECK_LAUNCH();
-      parts += blocks;
-    }
-    if (clip == 1 && tables.size() == 1 && parts <= JOIN_PARTS) {
-      hipLaunchKernelGGL((scale_joined<NORM>), dim3(parts), dim3(256), 0, s, tables[0], part, parts, max_norm, out);
+    hipLaunchKernelGGL((norm_parts<NORM, S>), grid, block, 0, s, t, part);
+    LDM_CHECK_LAUNCH();
+    if (clip == 1 && t.chunks > 0 && t.chunks <= JOIN_CHUNKS) {
+      hipLaunchKernelGGL((scale_joined<NORM, S>), grid, block, 0, s, t, part, (int)grid.x, max_norm, out);
       LDM_CHECK_LAUNCH();
       return LDM_OK;
     }
-    hipLaunchKernelGGL((norm_final<NORM>), dim3(1), dim3(256), 0, s, part, parts, max_norm, out);
+    hipLaunchKernelGGL((norm_final<NORM>), dim3(1), block, 0, s, part, (int)grid.x, max_norm, out);
     LDM_CHECK_LAUNCH();
   }
-  if (clip)
-    for (size_t i = tables.size(); i-- > 0;) {
-      const Table& t = tables[i];
-      hipLaunchKernelGGL(scale_all, dim3(std::min(t.chunks, MAX_BLOCKS)), dim3(256), 0, s, t, out);
-      LDM_CHECK_LAUNCH();
-    }
+  if (clip) {
+    hipLaunchKernelGGL((scale_all<S>), grid, block, 0, s, t, out);
+    LDM_CHECK_LAUNCH();
+  }
+  return LDM_OK;
+}
+template <typename S>
+int launch(const S& t, int norm_type, float max_norm, int clip, float* out, double* part, hipStream_t s) {
+  if (norm_type == LDM_NORM_2) return launch<LDM_NORM_2>(t, max_norm, clip, out, part, s);
+  if (norm_type == LDM_NORM_INF) return launch<LDM_NORM_INF>(t, max_norm, clip, out, part, s);
+  return launch<LDM_NORM_1>(t, max_norm, clip, out, part, s);
+}
+
+int launch_small(const SmallTable& t, int norm_type, float max_norm, int clip, float* out, hipStream_t s) {
+  const dim3 one(1), block(64 * SMALL_WAVES);
+  if (norm_type == LDM_NORM_2) hipLaunchKernelGGL((clip_small<LDM_NORM_2>), one, block, 0, s, t, max_norm, clip, out);
+  else if (norm_type == LDM_NORM_INF) hipLaunchKernelGGL((clip_small<LDM_NORM_INF>), one, block, 0, s, t, max_norm, clip, out);
+  else hipLaunchKernelGGL((clip_small<LDM_NORM_1>), one, block, 0, s, t, max_norm, clip, out);
+  LDM_CHECK_LAUNCH();
   return LDM_OK;
 }
 
 }  // namespace
 
+// partials, and behind them the chunk list where there may be more spans than a table holds (a span has one chunk
+// more than its whole ones at most, and a bf16 chunk has twice the elements)
 extern "C" size_t ldm_grad_norm_workspace_bytes(const int64_t* numel, int ntensors) {
   if (!numel || ntensors <= 0) return 0;
-  return (size_t)((entries_of(numel, ntensors) + TABLE - 1) / TABLE) * MAX_BLOCKS * sizeof(double);
+  size_t chunks = 0;
+  for (int i = 0; i < ntensors; ++i)
+    if (numel[i] > 0) chunks += (size_t)((numel[i] + chunk_of<float>() - 1) / chunk_of<float>());
+  return MAX_BLOCKS * sizeof(double) + (entries_of(numel, ntensors) > TABLE ? chunks * sizeof(Chunk) : 0);
 }
 
 extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, const uint8_t* dtypes, int ntensors,
@@ -217,8 +342,7 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
                              int64_t workspace_bytes, ldm_stream_t stream) {
   if (!ptrs || !numel || !dtypes || !out || ntensors <= 0 || clip < 0 || clip > 2) return LDM_ERR_ARG;
   if (norm_type < LDM_NORM_2 || norm_type > LDM_NORM_1 || !(max_norm >= 0.0)) return LDM_ERR_ARG;
-  const int64_t need = clip == 2 ? 0 : (int64_t)ldm_grad_norm_workspace_bytes(numel, ntensors);
-  if (need && (!workspace || workspace_bytes < need)) return LDM_ERR_ARG;
+  if (!workspace || workspace_bytes < (int64_t)ldm_grad_norm_workspace_bytes(numel, ntensors)) return LDM_ERR_ARG;
   // Tensors in the order of their addresses; those that lie back to back (views of a bucket) are one span.
   struct Span { uint64_t lo, hi, size; };
   std::vector<Span> spans;
@@ -242,6 +366,18 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
       else spans[++last] = spans[i];
     }
     if (!spans.empty()) spans.resize(last + 1);
+    int64_t units = 0;
+    for (const Span& p : spans) units += (int64_t)(p.hi - p.lo + 1023) / 1024;
+    if (clip != 2 && units <= UNITS * SMALL_WAVES && spans.size() <= SMALL_SPANS) {
+      SmallTable t;
+      t.units = 0;
+      for (size_t i = 0; i < spans.size(); ++i) {
+        const Span& p = spans[i];
+        t.e[i] = {p.lo | ((uint64_t)(p.size == 2) << 63), (uint32_t)((p.hi - p.lo) / p.size), (uint32_t)t.units};
+        for (int64_t k = (int64_t)(p.hi - p.lo + 1023) / 1024; k > 0; --k) t.span[t.units++] = (uint8_t)i;
+      }
+      return launch_small(t, norm_type, (float)max_norm, clip, out, reinterpret_cast<hipStream_t>(stream));
+    }
     for (const Span& p : spans) {
       const int64_t total = (int64_t)((p.hi - p.lo) / p.size);
       const int64_t chunk = p.size == 2 ? chunk_of<bf16_t>() : chunk_of<float>();
@@ -262,7 +398,22 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
   }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(workspace);
-  if (norm_type == LDM_NORM_2) return launch<LDM_NORM_2>(tables, (float)max_norm, clip, out, part, s);
-  if (norm_type == LDM_NORM_INF) return launch<LDM_NORM_INF>(tables, (float)max_norm, clip, out, part, s);
-  return launch<LDM_NORM_1>(tables, (float)max_norm, clip, out, part, s);
+  if (tables.size() <= 1) {
+    if (tables.empty()) {
+      tables.emplace_back();
+      tables[0].count = tables[0].chunks = 0;
+    }
+    return launch(tables[0], norm_type, (float)max_norm, clip, out, part, s);
+  }
+  Chunk* list = reinterpret_cast<Chunk*>(part + MAX_BLOCKS);
+  int64_t chunks = 0;
+  for (const Table& t : tables) chunks += t.chunks;
+  if (chunks > 0x7fffffff) return LDM_ERR_ARG;
+  chunks = 0;
+  for (const Table& t : tables) {
+    hipLaunchKernelGGL(list_chunks, dim3(t.count), dim3(64), 0, s, t, list + chunks);
+    LDM_CHECK_LAUNCH();
+    chunks += t.chunks;
+  }
+  return launch(ChunkList{list, (int)chunks}, norm_type, (float)max_norm, clip, out, part, s);
 }

@@ -373,7 +373,7 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int n = (int)ptrs.size();
   const OnDevice on(device);
   at::Tensor workspace;
-  const size_t bytes = clip == 2 ? 0 : p_norm_ws(numel.data(), n);
+  const size_t bytes = p_norm_ws(numel.data(), n);
   if (bytes) workspace = at::empty({(int64_t)bytes}, f32.dtype(at::kByte));
   const int rc = p_norm(ptrs.data(), numel.data(), codes.data(), n, (int)kind, max_norm, (int)clip,
                         out.data_ptr<float>(), bytes ? workspace.data_ptr() : nullptr, (int64_t)bytes, on.stream());
