@@ -177,7 +177,8 @@ __device__ __forceinline__ void chunk_scale(T* g, int n, F factor) {
   }, [&](int i, T v) { g[i] = from_f<T>(to_f(v) * f); });
 }
 
-// the last chunks first: the norm's pass has left them in the memory-side cache
+// the last chunks first: the norm's pass has left them in the memory-side cache (400 MB: 213 us, 244 us from the
+// front; 3.3 GB: no difference)
 template <typename S>
 __global__ __launch_bounds__(256) void scale_all(const S t, const float* __restrict__ out) {
   const float f = out[1];

@@ -418,31 +418,15 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
   LabelAt l;
   if (segments == 1) l = label_at<T>(a, pos);
   int bar = KEY_NONE;              // the wave's lists hold K keys that are no less
-  for (int base = seg * seg_len; base < end; base += 256 * N) {   // the same turns in every lane: they shuffle
-    const int at0 = base + tid * VEC;
-    Pack<T, VEC> v[UNR];
-    float f[N];
-#pragma unroll
-    for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + min(at0 + u * 256 * VEC, last));
+  auto turn = [&](int at0, float (&f)[N]) {
     bool odd = false;
-    float most = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < UNR; ++u) {
-      const int at = at0 + u * 256 * VEC, c0 = min(at, last);
-      Pack<uint8_t, VEC> m;
-      if (mask) m = load_pack<uint8_t, VEC>(mask + c0);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int i = u * VEC + j;
-        // only the row's last segment ends inside a block's reach, and its last pack reaches back over its neighbour
-        const bool in = at < end && c0 + j >= at && (!mask || m.v[j]);
-        f[i] = in ? to_f(v[u].v[j]) : -INFINITY;
-        odd |= f[i] != f[i];
-        most = fmaxf(most, f[i]);
-      }
-    }
+    for (int i = 0; i < N; ++i) odd |= f[i] != f[i];
     nan |= odd;
     if constexpr (K > 0) {
+      float most = f[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) most = fmaxf(most, f[i]);
       // a class enters only above the K-th key of some lane: later classes lose ties
       if (__any(odd || order_key(most) > bar)) {
 #pragma unroll
@@ -454,6 +438,35 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
       }
     }
     s.template add_all<N>(f, a.c2);
+  };
+  int base = seg * seg_len;        // the same turns in every lane: they exchange values
+  if (!mask)
+    for (; base + 256 * N <= end; base += 256 * N) {
+      Pack<T, VEC> v[UNR];
+      float f[N];
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + base + (u * 256 + tid) * VEC);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = to_f(v[i / VEC].v[i % VEC]);
+      turn(base + tid * VEC, f);
+    }
+  for (; base < end; base += 256 * N) {
+    const int at0 = base + tid * VEC;
+    Pack<T, VEC> v[UNR];
+    float f[N];
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + min(at0 + u * 256 * VEC, last));
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) {
+      const int at = at0 + u * 256 * VEC, c0 = min(at, last);
+      Pack<uint8_t, VEC> m;
+      if (mask) m = load_pack<uint8_t, VEC>(mask + c0);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        // only the row's last segment ends inside a block's reach, and its last pack reaches back over its neighbour
+        f[u * VEC + j] = at < end && c0 + j >= at && (!mask || m.v[j]) ? to_f(v[u].v[j]) : -INFINITY;
+    }
+    turn(at0, f);
   }
   int key = KEY_NONE, id = -1;
   if (!block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) return;
