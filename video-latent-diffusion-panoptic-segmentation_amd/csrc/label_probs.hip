@@ -399,14 +399,42 @@ __device__ __forceinline__ void finish_row(const Args& a, int64_t pos, const Lab
   if (lane < a.k) store_top(a, pos, lane, key, id, s, q.ls);
 }
 
-template <typename T, int VEC, int K>
+// A turn's classes enter the lanes' lists only above a bar: the K-th largest of the wave's lane maxima, or what an
+// earlier turn had; K classes at least are no less, and later ones lose ties.  So lists see little but the answer.
+template <int K, int N, typename C>
+__device__ __forceinline__ void enter_above_bar(Top<K>& top, int& bar, const float (&f)[N], bool odd, C class_of) {
+  if (bar == 0x7fffffff) return;
+  float most = f[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) most = fmaxf(most, f[i]);
+  int mine = odd ? 0x7fffffff : order_key(most);
+  if (!__any(mine > bar)) return;
+  int kth = KEY_NONE;
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    kth = wave_all(mine, KEY_NONE, Max());
+    if (kth <= bar) break;
+    if ((int)(threadIdx.x & 63) == __ffsll((unsigned long long)__ballot(mine == kth)) - 1) mine = KEY_NONE;
+  }
+  const float least = key_value(max(kth, bar + 1));
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (__any(!(f[i] < least)))
+      if (!(f[i] < least)) top.add(order_key(f[i]), class_of(i));
+  bar = max(bar, kth);
+}
+
+// WAVES = 1: a wave to a row, four rows to a block, for rows that a block's start and end would outweigh.
+template <typename T, int VEC, int K, int WAVES>
 __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, int seg_len, Part* __restrict__ parts,
                                                   int2* __restrict__ part_top) {
-  constexpr int UNR = 2, N = VEC * UNR;
-  __shared__ RowParts<K> sh;
-  const int64_t pos = segments == 1 ? blockIdx.x : blockIdx.x / segments;
+  constexpr int UNR = 2, N = VEC * UNR, W = 64 * WAVES;
+  __shared__ RowParts<WAVES == 4 ? K : 0> sh;
+  const int64_t pos = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)
+                                 : segments == 1 ? blockIdx.x : blockIdx.x / segments;
+  if (WAVES == 1 && pos >= a.positions) return;
   const int seg = segments == 1 ? 0 : (int)(blockIdx.x - pos * segments);
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x & (W - 1), lane = tid & 63;
   const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
   const uint8_t* mask = a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
   const int end = min(a.classes, (seg + 1) * seg_len), last = a.classes - VEC;
@@ -414,51 +442,40 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
   s.clear();
   Top<K> top;
   top.clear();
-  bool nan = false;
+  uint64_t nans = 0;               // lanes that saw one
   LabelAt l;
   if (segments == 1) l = label_at<T>(a, pos);
   int bar = KEY_NONE;              // the wave's lists hold K keys that are no less
   auto turn = [&](int at0, float (&f)[N]) {
-    bool odd = false;
+    uint64_t odd = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) odd |= f[i] != f[i];
-    nan |= odd;
-    if constexpr (K > 0) {
-      float most = f[0];
-#pragma unroll
-      for (int i = 1; i < N; ++i) most = fmaxf(most, f[i]);
-      // a class enters only above the K-th key of some lane: later classes lose ties
-      if (__any(odd || order_key(most) > bar)) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int k = order_key(f[i]);
-          if (k > bar) top.add(k, min(at0 + i / VEC * 256 * VEC, last) + i % VEC);
-        }
-        bar = wave_all(top.key[K - 1], KEY_NONE, Max());
-      }
-    }
+    for (int i = 0; i < N; i += 2) odd |= __ballot(__builtin_isunordered(f[i], f[i + 1]));
+    nans |= odd;
+    if constexpr (K > 0)
+      enter_above_bar<K, N>(top, bar, f, odd >> lane & 1,
+                            [&](int i) { return min(at0 + i / VEC * W * VEC, last) + i % VEC; });
     s.template add_all<N>(f, a.c2);
   };
   int base = seg * seg_len;        // the same turns in every lane: they exchange values
   if (!mask)
-    for (; base + 256 * N <= end; base += 256 * N) {
+    for (; base + W * N <= end; base += W * N) {
       Pack<T, VEC> v[UNR];
       float f[N];
 #pragma unroll
-      for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + base + (u * 256 + tid) * VEC);
+      for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + base + (u * W + tid) * VEC);
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = to_f(v[i / VEC].v[i % VEC]);
       turn(base + tid * VEC, f);
     }
-  for (; base < end; base += 256 * N) {
+  for (; base < end; base += W * N) {
     const int at0 = base + tid * VEC;
     Pack<T, VEC> v[UNR];
     float f[N];
 #pragma unroll
-    for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + min(at0 + u * 256 * VEC, last));
+    for (int u = 0; u < UNR; ++u) v[u] = load_pack<T, VEC>(x + min(at0 + u * W * VEC, last));
 #pragma unroll
     for (int u = 0; u < UNR; ++u) {
-      const int at = at0 + u * 256 * VEC, c0 = min(at, last);
+      const int at = at0 + u * W * VEC, c0 = min(at, last);
       Pack<uint8_t, VEC> m;
       if (mask) m = load_pack<uint8_t, VEC>(mask + c0);
 #pragma unroll
@@ -469,13 +486,20 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
     turn(at0, f);
   }
   int key = KEY_NONE, id = -1;
-  if (!block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) return;
-  if (segments == 1) {
+  bool nan = nans != 0;
+  if constexpr (WAVES == 1) {
+    s = wave_join(s, a.c2);
+    if constexpr (K > 0) wave_top<K>(top, a.k, key, id);
     finish_row(a, pos, l, s, nan, key, id);
-    return;
+  } else {
+    if (!block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) return;
+    if (segments == 1) {
+      finish_row(a, pos, l, s, nan, key, id);
+      return;
+    }
+    if (lane == 0) parts[blockIdx.x] = {s.m, s.r, s.t, nan};
+    if (lane < a.k) part_top[(int64_t)blockIdx.x * a.k + lane] = make_int2(key, id);
   }
-  if (lane == 0) parts[blockIdx.x] = {s.m, s.r, s.t, nan};
-  if (lane < a.k) part_top[(int64_t)blockIdx.x * a.k + lane] = make_int2(key, id);
 }
 
 // one block per row: its segments in the order of their classes
@@ -847,6 +871,7 @@ int launch_planes(const Args& a, hipStream_t s) {
   return LDM_OK;
 }
 
+constexpr int WAVE_CLASSES = 8192;       // a wave's row
 constexpr int SHORT_CLASSES = 1024;      // at most 16 classes in a lane's registers
 // segments of a long row: whole multiples of a block's reach, 512 blocks at least where rows are few
 int segments_of(int64_t positions, int64_t classes, int dtype) {
@@ -866,10 +891,15 @@ void launch_short(const Args& a, hipStream_t s) {
 template <typename T, int K>
 void launch_long_as(const Args& a, int segments, void* ws, hipStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
+  if (a.positions >= 2048 && a.classes <= WAVE_CLASSES) {
+    hipLaunchKernelGGL((probs_rows<T, VEC, K, 1>), dim3((unsigned)((a.positions + 3) / 4)), dim3(256), 0, s, a, 1,
+                       a.classes, (Part*)nullptr, (int2*)nullptr);
+    return;
+  }
   const int reach = 256 * VEC, per = ((a.classes + reach - 1) / reach + segments - 1) / segments;
   Part* parts = (Part*)ws;
   int2* tops = (int2*)(parts + a.positions * segments);
-  hipLaunchKernelGGL((probs_rows<T, VEC, K>), dim3((unsigned)(a.positions * segments)), dim3(256), 0, s, a, segments,
+  hipLaunchKernelGGL((probs_rows<T, VEC, K, 4>), dim3((unsigned)(a.positions * segments)), dim3(256), 0, s, a, segments,
                      per * reach, parts, tops);
   if (segments > 1)
     hipLaunchKernelGGL((probs_join<T, K>), dim3((unsigned)a.positions), dim3(256), 0, s, a, segments, parts, tops);
