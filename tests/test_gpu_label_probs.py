@@ -346,3 +346,98 @@ def test_streams_and_graphs():
             assert torch.equal(gd, d)
     for (o, d), c in zip(on_side, cases):
         assert o.log_prob.isfinite().all() and d.isfinite().all()
+
+
+def test_panoptic_head_reports_entropy_and_alternatives():
+    """postprocess_panoptic(alternatives=k): the statistics are those of the head's own logits, the first alternative
+    is the label before thresholds, and what it returned before is unchanged."""
+    from ldmseg.pipelines.panoptic import postprocess_panoptic
+    g = torch.Generator().manual_seed(12)
+    lo = (torch.randn(2, 19, 12, 20, generator=g) * 4).to(DEV)
+    pad = torch.zeros(2, 48, 80, dtype=torch.bool, device=DEV)
+    pad[:, :41, 3:77] = True
+    args = (lo, (48, 80), pad, [(83, 147), (41, 74)], 0.5, 20, 0.5, 255)
+    plain = postprocess_panoptic(*args)
+    more = postprocess_panoptic(*args, alternatives=3)
+    bare = postprocess_panoptic(*args, alternatives=0)
+    for i, (a, b, c) in enumerate(zip(plain, more, bare)):
+        assert set(a) == {"panoptic_seg", "cleaned_pred"} and set(c) == set(a) | {"entropy"}
+        assert torch.equal(a["cleaned_pred"], b["cleaned_pred"]) and torch.equal(b["entropy"], c["entropy"])
+        assert torch.equal(a["panoptic_seg"][0], b["panoptic_seg"][0])
+        m = K.resize_bilinear(lo, size=(48, 80))[i:i + 1, :, :41, 3:77]
+        m = K.resize_bilinear(m, size=args[3][i])
+        ref = oracle.label_log_probs(m, topk=3)
+        ids, lp = b["alternatives"]
+        assert torch.equal(ids.long().cpu(), ref["top_ids"][0])
+        assert (lp.double().cpu() - ref["top_log_probs"][0]).abs().max() < 2e-5
+        assert (b["entropy"].double().cpu() - ref["entropy"][0]).abs().max() < 2e-5
+        kept = b["cleaned_pred"] >= 0
+        assert torch.equal(b["cleaned_pred"][kept], ids[0].long()[kept])
+
+
+def test_training_step_of_both_operators():
+    """Loss, gradient, norm and clip together, as a training loop uses them: a small head on bf16 features, its loss the
+    labels' log probability and an entropy term, two steps of SGD; against the same in 64 bits."""
+    from ldmseg.trainers import clip_grad_norm_
+    g = torch.Generator().manual_seed(21)
+    B, D, C, H, W, limit, lr = 3, 16, 30, 17, 23, 0.05, 0.5
+    feats = torch.randn(B, D, H, W, generator=g)
+    y = _labels((B, H, W), C, g)
+    y[0, 0, :3] = 7
+    w0, b0 = torch.randn(C, D, generator=g) * 0.3, torch.randn(C, generator=g) * 0.1
+    n = (y != IGN).sum().item()
+
+    head = torch.nn.Conv2d(D, C, 1).to(DEV)
+    with torch.no_grad():
+        head.weight.copy_(w0.view(C, D, 1, 1))
+        head.bias.copy_(b0)
+    rw, rb = w0.double().requires_grad_(), b0.double().requires_grad_()
+    x, yd = feats.to(DEV), y.to(DEV)
+    for step in range(2):
+        logits = torch.nn.functional.conv2d(x, head.weight, head.bias)
+        out = ops.label_log_probs(logits, yd, ignore_label=IGN)
+        (-out.log_prob.sum() / n - 0.01 * out.entropy.mean()).backward()
+        norm = clip_grad_norm_(head.parameters(), limit)
+
+        z = torch.einsum("bdhw,cd->bchw", feats.double(), rw) + rb.view(1, C, 1, 1)
+        lp = torch.log_softmax(z, 1)
+        ent = -(lp.exp() * lp).sum(1)
+        nll = -lp.gather(1, y.clamp(max=C - 1)[:, None])[:, 0][y != IGN].sum() / n
+        gw, gb = torch.autograd.grad(nll - 0.01 * ent.mean(), (rw, rb))
+        rn = torch.sqrt(gw.square().sum() + gb.square().sum())
+        assert rn > limit and abs(norm.item() - rn.item()) < 1e-4 * rn.item()
+        f = limit / (rn + 1e-6)
+        # fp32 products of 16 terms and sums of 1173 positions in torch's convolution: a few 1e-5 relative to the norm
+        assert (head.weight.grad.view(C, D).double().cpu() - gw * f).abs().max() < 1e-4 * limit
+        assert (head.bias.grad.double().cpu() - gb * f).abs().max() < 1e-4 * limit
+        with torch.no_grad():
+            for p in head.parameters():
+                p.sub_(p.grad, alpha=lr)
+                p.grad = None
+            rw -= lr * f * gw
+            rb -= lr * f * gb
+
+
+def test_clipping_the_drop_in_unet():
+    """loss.backward() through the drop-in UNet's autograd node leaves one fp32 tensor per parameter: clip_grad_norm_
+    clips them as torch's own does."""
+    from ldmseg.models import UNet
+    from ldmseg.trainers import clip_grad_norm_
+    torch.manual_seed(0)
+    u = UNet(block_out_channels=(64, 128, 128, 128), cross_attention_dim=None)
+    u.modify_encoder(in_channels=8, init_mode_seg="copy", init_mode_image="random")
+    u.freeze_layers(["time_embedding"])
+    u = u.to(DEV).train()
+    out = u(torch.randn(1, 8, 16, 16, device=DEV), torch.tensor([500], device=DEV)).sample
+    out.square().mean().backward()
+    ps = [p for p in u.parameters() if p.grad is not None]
+    assert len(ps) > 200
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    for p, q in zip(ps, twin):
+        q.grad = p.grad.clone()
+    nt = torch.nn.utils.clip_grad_norm_(twin, 1e-3)
+    n = clip_grad_norm_(u.parameters(), 1e-3)
+    assert n > 1e-3 and abs(n.item() - nt.item()) <= 1e-5 * nt.item()
+    for p, q in zip(ps, twin):
+        torch.testing.assert_close(p.grad, q.grad, rtol=2e-5, atol=0)
+    assert abs(K.grad_norm([p.grad for p in ps]).item() - 1e-3) < 1e-6

@@ -150,16 +150,18 @@ __device__ __forceinline__ DdimCoef ddim_coef(const float* ac, int64_t t, int st
   const float bt = 1.0f - at;
   return DdimCoef{sqrtf(at), sqrtf(bt), sqrtf(ap), sqrtf(1.0f - ap)};
 }
-// m = model output, x = sample -> (prev_sample, pred_original_sample)
+// m = model output, x = sample -> (prev_sample, pred_original_sample).  Which product of a sum is fused is written
+// out, so that every kernel that includes this gives the same bits whatever its compiler flags choose.
 __device__ __forceinline__ float2 ddim_apply(const DdimCoef& c, float m, float x, int pred, int clip, float clip_range,
                                              int use_clipped) {
+#pragma clang fp contract(off)
   float x0, eps;
-  if (pred == LDM_PRED_EPSILON) { x0 = (x - c.sb * m) / c.sa; eps = m; }
-  else if (pred == LDM_PRED_SAMPLE) { x0 = m; eps = (x - c.sa * x0) / c.sb; }
-  else { x0 = c.sa * x - c.sb * m; eps = c.sa * m + c.sb * x; }
+  if (pred == LDM_PRED_EPSILON) { x0 = fmaf(-c.sb, m, x) / c.sa; eps = m; }
+  else if (pred == LDM_PRED_SAMPLE) { x0 = m; eps = fmaf(-c.sa, x0, x) / c.sb; }
+  else { x0 = fmaf(c.sa, x, -(c.sb * m)); eps = c.sa * m + c.sb * x; }
   if (clip) x0 = fminf(fmaxf(x0, -clip_range), clip_range);
-  if (use_clipped) eps = (x - c.sa * x0) / c.sb;
-  return make_float2(c.sap * x0 + c.sbp * eps, x0);
+  if (use_clipped) eps = fmaf(-c.sa, x0, x) / c.sb;
+  return make_float2(fmaf(c.sap, x0, c.sbp * eps), x0);
 }
 
 #define LDM_CHECK_LAUNCH()                                   \

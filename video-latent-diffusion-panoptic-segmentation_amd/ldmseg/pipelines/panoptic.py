@@ -40,12 +40,16 @@ def _crop_box(padding_mask):
 
 
 def postprocess_panoptic(masks_logits, image_hw, padding_masks, orig_sizes, mask_th, count_th, overlap_th,
-                         ignore_label, threshold_output=True, threshold_mode="max"):
+                         ignore_label, threshold_output=True, threshold_mode="max", alternatives=None):
     """compute_pq's per-batch post-processing (:1276-1330) on the GPU.
 
     masks_logits fp32 [B, K, Hd, Wd] (decode_latents(return_logits=True)); image_hw = the RGB
     input size; padding_masks [B, Hi, Wi]; orig_sizes [(h, w)] per image.  Returns, per image,
-    ``{"panoptic_seg": (cleaned + 1, segments_info), "cleaned_pred": cleaned}`` (GPU int64)."""
+    ``{"panoptic_seg": (cleaned + 1, segments_info), "cleaned_pred": cleaned}`` (GPU int64).
+
+    ``alternatives`` (an opt-in this build adds): k >= 0 also reports how sure the head is of every pixel, from the
+    same logits: "entropy" fp32 [h, w] (nats) and, for k > 0, "alternatives": (ids int32 [k, h, w], log
+    probabilities fp32 [k, h, w]), the most likely label first."""
     x = K.resize_bilinear(masks_logits.float(), size=tuple(image_hw))
     results = []
     for i in range(x.shape[0]):
@@ -55,6 +59,11 @@ def postprocess_panoptic(masks_logits, image_hw, padding_masks, orig_sizes, mask
         cleaned, keep = panoptic_head(m, mask_th, count_th, overlap_th, ignore_label, threshold_output,
                                       threshold_mode)
         results.append({"panoptic_seg": (cleaned[0] + 1, segments_info(keep[0])), "cleaned_pred": cleaned[0]})
+        if alternatives is not None:
+            p = K.label_log_probs(m, topk=alternatives)
+            results[-1]["entropy"] = p.entropy[0]
+            if alternatives:
+                results[-1]["alternatives"] = (p.top_ids[0], p.top_log_probs[0])
     return results
 
 

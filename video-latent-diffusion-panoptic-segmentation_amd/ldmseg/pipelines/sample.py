@@ -12,10 +12,11 @@ from .panoptic import postprocess_panoptic
 def sample_panoptic(rgb_images, vae_image, vae_semseg, unet, scheduler, *, rgb_size=192, latent_size=64,
                     num_inference_steps=50, seed=0, self_condition=False, mask_th=0.5, count_th=512,
                     overlap_th=0.5, ignore_label=255, threshold_output=True, threshold_mode="max",
-                    padding_masks=None, orig_sizes=None, use_graph=True, stepper=None):
+                    padding_masks=None, orig_sizes=None, use_graph=True, stepper=None, alternatives=None):
     """rgb_images fp32 [B, 3, H, W] in [0, 1] (GPU; B = the T frames of a clip) -> per frame
     {"panoptic_seg": (ids [h, w] int64, segments_info), "cleaned_pred": ...}.
-    ``stepper``: a prepared DenoiseStep to reuse (its HIP graph) across clips of one shape."""
+    ``stepper``: a prepared DenoiseStep to reuse (its HIP graph) across clips of one shape.
+    ``alternatives``: postprocess_panoptic's per-pixel entropy and most likely labels."""
     B, _, H, W = rgb_images.shape
     rgb_latents, _ = encode_inputs(rgb_images, vae_image.encode, vae_image.scaling_factor, latent_size,
                                    resize=rgb_size, weight_dtype=vae_image.dtype)          # :1230-1236
@@ -29,4 +30,4 @@ def sample_panoptic(rgb_images, vae_image, vae_semseg, unet, scheduler, *, rgb_s
     if orig_sizes is None:
         orig_sizes = [(H, W)] * B
     return postprocess_panoptic(logits, (H, W), padding_masks, orig_sizes, mask_th, count_th, overlap_th,
-                                ignore_label, threshold_output, threshold_mode)          # :1262-1330
+                                ignore_label, threshold_output, threshold_mode, alternatives)          # :1262-1330
