@@ -53,7 +53,7 @@ def _check(params, max_norm, kind=2.0):
 SIZES = {
     "one": [1], "two": [2], "odd": [3, 1, 7, 63, 65], "edges": [255, 256, 257, 8191, 8192, 8193],
     "many": [1 + (i * 37) % 301 for i in range(700)], "table_full": [5] * 224, "table_over": [5] * 225,
-    "large": [3_000_001, 17, 2_097_152, 0, 9], "zero_sized": [0, 4, 0], "only_zero_sized": [0, 0],
+    "listed_long": [40_001] * 300, "large": [3_000_001, 17, 2_097_152, 0, 9], "zero_sized": [0, 4, 0], "only_zero_sized": [0, 0],
     "around_one_block": [16_384, 16_383, 1], "around_one_block_over": [32_768, 1, 32_769],
 }
 
@@ -156,6 +156,23 @@ def test_non_finite_and_extreme_values(dtype):
     # all zeros: the norm is 0, the factor 1
     ps = grads(0.0)
     assert clip_grad_norm_(ps, 1.0) == 0 and (ps[0].grad == 0).all()
+
+
+def test_clipping_is_seen_by_autograd():
+    """A gradient that a graph has saved is modified in place: the graph's backward refuses, as after torch's clip."""
+    p = torch.nn.Parameter(torch.ones(4, device=DEV))
+    p.grad = torch.full((4,), 3.0, device=DEV)
+    w = torch.ones(4, device=DEV, requires_grad=True)
+    y = (w * p.grad).sum()
+    assert abs(K.grad_norm(p.grad).item() - 6.0) < 1e-6        # a tensor alone is a list of one; reading changes nothing
+    clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        q = torch.ones(3, device=DEV)
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        K.clip_grads([q], 1.0)
+    assert (q == 1).all()
 
 
 def test_a_gradient_listed_twice_is_refused():

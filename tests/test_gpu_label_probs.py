@@ -441,3 +441,31 @@ def test_clipping_the_drop_in_unet():
     for p, q in zip(ps, twin):
         torch.testing.assert_close(p.grad, q.grad, rtol=2e-5, atol=0)
     assert abs(K.grad_norm([p.grad for p in ps]).item() - 1e-3) < 1e-6
+
+
+def test_mask_rows_that_do_not_divide_the_positions():
+    """The C entry takes any number of positions to a mask row: the last row's may be fewer, and nothing behind the
+    last position is written."""
+    import ctypes
+    g = torch.Generator().manual_seed(9)
+    C, N, div = 20, 330, 128                        # rows of 128, 128 and 74 positions
+    x = torch.randn(C, N, generator=g).to(DEV)
+    m = (torch.rand(3, C, generator=g) < 0.5).to(DEV)
+    m[:, 3] = True
+    ent, stats = torch.full((N + 300,), 7.0, device=DEV), torch.full((4 * N + 300,), 7.0, device=DEV)
+    d = torch.full((C * N + 300,), 7.0, device=DEV)
+    ge = torch.randn(N, generator=g).to(DEV)
+    lib, st = K.load_library(), torch.cuda.current_stream().cuda_stream
+    common = dict(logits=x.data_ptr(), n0=1, n1=1, n2=N, s2=1, classes=C, sc=N, class_mask=m.data_ptr(), mask_stride=C,
+                  mask_div=div, temperature=1.0, dtype=0)
+    p = K.LabelProbsParams(**common, inner=N, entropy=ent.data_ptr(), stats=stats.data_ptr())
+    assert lib.ldm_label_log_probs(ctypes.byref(p), st) == 0
+    b = K.LabelProbsBwdParams(**common, stats=stats.data_ptr(), d_entropy=ge.data_ptr(), d_logits=d.data_ptr(), o2=1, oc=N)
+    assert lib.ldm_label_log_probs_bwd(ctypes.byref(b), st) == 0
+    for r in range(3):
+        s = slice(r * div, min(N, (r + 1) * div))
+        ref = oracle.label_log_probs(x[:, s], dim=0, class_mask=m[r])
+        assert (ent[s].double().cpu() - ref["entropy"]).abs().max() < 1e-5
+        want = oracle.label_log_probs_bwd(x[:, s], None, None, ge[s], dim=0, class_mask=m[r])
+        assert (d[:C * N].view(C, N)[:, s].double().cpu() - want).abs().max() < 1e-5
+    assert (ent[N:] == 7).all() and (stats[4 * N:] == 7).all() and (d[C * N:] == 7).all()

@@ -70,6 +70,9 @@ def test_c_entries_refuse_before_any_launch():
                 dict(class_mask=16, mask_div=0), dict(class_mask=16, mask_div=4, mask_stride=-1)):
         p = K.LabelProbsParams(**{**ok, **bad})
         assert lib.ldm_label_log_probs(ctypes.byref(p), None) == 1, bad
+    for big in (dict(n2=1 << 32, inner=(1 << 32) + 256), dict(n2=1 << 26, sc=1, s2=600, classes=600, inner=1),
+                dict(n2=1 << 24, sc=1, s2=9000, classes=9000, inner=1), dict(n2=1 << 27, sc=1, s2=3000, classes=3000, inner=1)):
+        assert lib.ldm_label_log_probs(ctypes.byref(K.LabelProbsParams(**{**ok, **big, "n2": big["n2"] + 256})), None) == 1
     assert lib.ldm_label_log_probs(None, None) == 1
     assert lib.ldm_label_log_probs(ctypes.byref(K.LabelProbsParams(**{**ok, "n2": 0})), None) == 0
     okb = dict(n0=1, n1=1, n2=4, s2=1, classes=5, sc=4, o2=1, oc=4, temperature=1.0, dtype=0, logits=16, stats=16,

@@ -602,11 +602,11 @@ __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling t
   const unsigned row = LISTED ? blockIdx.x / tile.blocks : 0;
   const int64_t block = LISTED ? blockIdx.x - row * tile.blocks : blockIdx.x;
   const int64_t want = SPLIT ? block * 64 + lane : block * 256 + threadIdx.x;
-  const bool live = want < tile.run;
+  const bool live = want < tile.run && row * tile.run + want < a.positions;
   int n = a.classes;
   if (LISTED) n = list_classes(a.mask + row * a.mask_stride, a.classes, list);
   if (!SPLIT && !live) return;
-  const int64_t pos = row * tile.run + (live ? want : tile.run - 1);
+  const int64_t pos = live ? row * tile.run + want : a.positions - 1;
   const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
   const uint8_t* mask = a.mask ? a.mask + (LISTED ? row : pos / a.mask_div) * a.mask_stride : nullptr;
   const int c0 = SPLIT ? (int)((int64_t)n * wave >> 2) : 0;
@@ -752,8 +752,8 @@ __global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, cons
     const int c = c0 + (int)(threadIdx.x & 63);
     bits = __ballot(c < c1 && a.mask[row * a.mask_stride + c]);
   }
-  if (want >= tile.run) return;
   const int64_t pos = row * tile.run + want;
+  if (want >= tile.run || pos >= a.positions) return;
   const T* x = a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
   T* dx = a.dx + offset_of(pos, a.n1, a.n2, a.o0, a.o1, a.o2);
   const uint8_t* mask = !UNIFORM && a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
@@ -824,8 +824,11 @@ __global__ __launch_bounds__(256) void probs_bwd_rows(const BwdArgs<T> a, unsign
 bool bad_positions(int64_t n0, int64_t n1, int64_t n2, int64_t classes, int64_t* n) {
   if (n0 < 0 || n1 < 0 || n2 < 0 || classes <= 0 || classes > (1 << 30)) return true;
   *n = n0 * n1 * n2;
-  return *n > (1LL << 38);                      // grids stay below 2^31 blocks of 256
+  return *n > (1LL << 38);
 }
+
+// A launch has less than 2^32 threads, blocks of 256 here; a call that would need more is refused.
+constexpr int64_t MOST_BLOCKS = (1LL << 24) - 1;
 
 // whether whole blocks of positions can share a row of the class mask, and the runs then
 bool mask_runs(const void* mask, int64_t mask_div, int64_t positions, int per_block, Tiling* t, int64_t* rows) {
@@ -837,7 +840,7 @@ bool mask_runs(const void* mask, int64_t mask_div, int64_t positions, int per_bl
     *rows = (positions + mask_div - 1) / mask_div;
   }
   t->blocks = (unsigned)((t->run + per_block - 1) / per_block);
-  return mask != nullptr;
+  return mask && *rows * t->blocks <= MOST_BLOCKS;
 }
 
 template <typename T, int K, bool SPLIT>
@@ -861,6 +864,7 @@ void launch_planes_split(const Args& a, hipStream_t s) {
 }
 template <typename T>
 int launch_planes(const Args& a, hipStream_t s) {
+  if ((a.positions + 255) / 256 > MOST_BLOCKS) return LDM_ERR_ARG;
   if (a.k == 0) launch_planes_split<T, 0>(a, s);
   else if (a.k == 1) launch_planes_split<T, 1>(a, s);
   else if (a.k == 2) launch_planes_split<T, 2>(a, s);
@@ -910,15 +914,15 @@ int launch(const Args& a, void* ws, hipStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   if (a.sc == 1 && a.classes > SHORT_CLASSES) {
     const int segments = segments_of(a.positions, a.classes, sizeof(T) == 2 ? LDM_BF16 : LDM_F32);
-    if (a.positions * segments > 0x7fffffff) return LDM_ERR_ARG;
+    if ((a.classes <= WAVE_CLASSES ? (a.positions + 3) / 4 : a.positions * segments) > MOST_BLOCKS) return LDM_ERR_ARG;
     if (a.k == 0) launch_long_as<T, 0>(a, segments, ws, s);
     else if (a.k == 1) launch_long_as<T, 1>(a, segments, ws, s);
     else if (a.k <= 4) launch_long_as<T, 4>(a, segments, ws, s);
     else if (a.k <= 8) launch_long_as<T, 8>(a, segments, ws, s);
     else launch_long_as<T, 16>(a, segments, ws, s);
   } else if (a.sc == 1 && a.classes >= VEC) {
-    if (a.positions > (1LL << 32)) return LDM_ERR_ARG;
     const int lanes = (a.classes + 15) / 16;
+    if ((a.positions * lanes + 127) / 128 > MOST_BLOCKS) return LDM_ERR_ARG;      // lanes round up to a power of two
     if (lanes <= 1) launch_short<T, 1>(a, s);
     else if (lanes <= 2) launch_short<T, 2>(a, s);
     else if (lanes <= 4) launch_short<T, 4>(a, s);
@@ -949,11 +953,11 @@ int launch_bwd(const ldm_label_probs_bwd_params* p, int64_t n, hipStream_t s) {
     const unsigned per_row = (unsigned)((a.classes + RV - 1) / RV);
     if (per_row < 256) {
       const int64_t blocks = (n * per_row + 255) / 256;
-      if (blocks > 0x7fffffff) return LDM_ERR_ARG;
+      if (blocks > MOST_BLOCKS) return LDM_ERR_ARG;
       hipLaunchKernelGGL((probs_bwd_rows<T, RV, 1, true>), dim3((unsigned)blocks), dim3(256), 0, s, a, per_row, 1u);
     } else {
       const unsigned bpr = (per_row + 511) / 512;
-      if (n * bpr > 0x7fffffff) return LDM_ERR_ARG;
+      if (n * bpr > MOST_BLOCKS) return LDM_ERR_ARG;
       hipLaunchKernelGGL((probs_bwd_rows<T, RV, 2, false>), dim3((unsigned)(n * bpr)), dim3(256), 0, s, a, per_row, bpr);
     }
     LDM_CHECK_LAUNCH();
@@ -963,7 +967,7 @@ int launch_bwd(const ldm_label_probs_bwd_params* p, int64_t n, hipStream_t s) {
   int span = 32;
   while (span > 8 && n / 64 * ((a.classes + span - 1) / span) < 12 * 256) span /= 2;
   const unsigned spans = (unsigned)((a.classes + span - 1) / span);
-  if (spans > 65535) return LDM_ERR_ARG;
+  if (spans > 65535 || (n + 255) / 256 > MOST_BLOCKS) return LDM_ERR_ARG;
   Tiling t;
   int64_t rows;
   if (mask_runs(a.mask, a.mask_div, n, 256, &t, &rows)) {

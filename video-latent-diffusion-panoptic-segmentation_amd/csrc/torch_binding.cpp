@@ -363,6 +363,7 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     TORCH_CHECK_VALUE(g.device() == device, "gradients on ", device, " and ", g.device(), ": one device per call");
     TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense() || g.numel() == 0,
                       "a gradient is no dense memory (an expanded or strided view): make it contiguous");
+    if (clip) g.unsafeGetTensorImpl()->bump_version();       // written in place: autograd sees it
     numel.push_back(g.numel());
     ptrs.push_back(g.numel() ? g.data_ptr() : nullptr);
   }

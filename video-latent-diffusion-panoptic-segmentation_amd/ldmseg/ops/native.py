@@ -1930,6 +1930,8 @@ NORM_TYPES = {2.0: 0, math.inf: 1, 1.0: 2}
 def _grad_norm(tensors, of_params, norm_type, max_norm, clip, out=None):
     """(norm, [norm, factor]) of tensors, or of their gradients; None where there are none.  ``clip`` as in
     ldm_grad_norm."""
+    if isinstance(tensors, torch.Tensor):
+        tensors = (tensors,)
     kind = NORM_TYPES.get(norm_type)
     if kind is None:
         raise ValueError(f"norm_type must be 2, inf or 1, got {norm_type}")

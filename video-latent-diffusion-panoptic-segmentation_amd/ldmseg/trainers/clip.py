@@ -15,13 +15,11 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     dense fp32 or bf16 on one GPU, in any mix; norm_type 2, inf or 1.  A non-finite norm scales by its
     factor as torch does (inf: 0, NaN: NaN) unless ``error_if_nonfinite``, which raises before anything is
     scaled and is the only form that waits for the GPU.  A gradient listed twice is refused."""
-    if isinstance(parameters, torch.Tensor):
-        parameters = (parameters,)
     norm_type = float(norm_type)
     if not error_if_nonfinite:
         r = K._grad_norm(parameters, True, norm_type, max_norm, 1)
         return torch.tensor(0.0) if r is None else r[0]
-    parameters = list(parameters)
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     r = K._grad_norm(parameters, True, norm_type, max_norm, 0)
     if r is None:
         return torch.tensor(0.0)
