@@ -350,20 +350,84 @@ __global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
 // in flight.  One segment to a row: the block finishes it.  More: what the segments come to goes to the workspace
 // and probs_join finishes the row.
 struct Part { float m, r, t; int nan; };
-template <int K>
+// (key, class) as one number: larger is earlier in the answer (larger key, then lower class), 0 is none
+__device__ __forceinline__ uint64_t candidate(int key, int id) {
+  return id < 0 ? 0 : (uint64_t)(uint32_t)(key ^ (int)0x80000000) << 32 | (uint32_t)~id;
+}
+// A wave's share of the candidates for its row's answer, at most CAP of them, written to `to`: the entries of the
+// lanes' lists that are no less than `bar` (which holds the wave's n first), or just those n if there are more.
+template <int K, int CAP>
+__device__ __forceinline__ int wave_candidates(Top<K>& top, int bar, int n, uint64_t* to) {
+  const int lane = threadIdx.x & 63;
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const bool in = top.id[i] >= 0 && top.key[i] >= bar;
+    const uint64_t who = __ballot(in);
+    if (!who) break;
+    const int more = __popcll(who);
+    if (count + more > CAP) {
+      int key, id;
+      wave_top<K>(top, n, key, id);
+      if (lane < n) to[lane] = candidate(key, id);
+      return __popcll(__ballot(lane < n && id >= 0));
+    }
+    if (in) to[count + __popcll(who & ((1ull << lane) - 1))] = candidate(top.key[i], top.id[i]);
+    count += more;
+  }
+  return count;
+}
+// The n <= 16 first of a wave's candidates (0: none) in their order, candidates being in runs of `count` at every
+// 64 / RUNS lanes: each finds its place by counting those before it.  Lane j < n gets the j-th.
+template <int RUNS>
+__device__ __forceinline__ void first_of(uint64_t mine, const int (&count)[RUNS], int n, uint64_t* sorted, int& key,
+                                         int& id) {
+  const int lane = threadIdx.x & 63;
+  int place = 0;
+#pragma unroll
+  for (int w = 0; w < RUNS; ++w)
+    for (int j = 0; j < count[w]; ++j) {
+      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), w * (64 / RUNS) + j) << 32 |
+                             (uint32_t)__builtin_amdgcn_readlane((int)mine, w * (64 / RUNS) + j);
+      place += other > mine;
+    }
+  if (lane < 16) sorted[lane] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (mine && place < n) sorted[place] = mine;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const uint64_t r = lane < n ? sorted[lane] : 0;
+  key = r ? (int)(r >> 32) ^ (int)0x80000000 : KEY_NONE;
+  id = r ? (int)~(uint32_t)r : -1;
+}
+// the K-th largest of the wave's lane values, or what is above none of them
+template <int K> __device__ __forceinline__ int kth_largest(int mine, int floor) {
+  int kth = KEY_NONE;
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    kth = wave_all(mine, KEY_NONE, Max());
+    if (kth <= floor) break;
+    if ((int)(threadIdx.x & 63) == __ffsll((unsigned long long)__ballot(mine == kth)) - 1) mine = KEY_NONE;
+  }
+  return kth;
+}
+
+template <int K, int WAVES>
 struct RowParts {
-  Soft part[4];
-  int nan[4], key[K > 0 ? 64 : 1], id[K > 0 ? 64 : 1];
+  Soft part[WAVES];
+  int nan[WAVES], count[WAVES];
+  uint64_t cand[K > 0 ? 64 : 1], sorted[K > 0 ? 16 : 1];
 };
 // the block's threads' sums and lists joined, in wave 0 (lane j < k: the j-th of the list); other waves get nothing
 template <int K>
-__device__ __forceinline__ bool block_join_row(RowParts<K>& sh, Soft& s, Top<K>& top, bool& nan, int k, float c2,
-                                               int& key, int& id) {
+__device__ __forceinline__ bool block_join_row(RowParts<K, 4>& sh, Soft& s, Top<K>& top, int bar, bool& nan, int k,
+                                               float c2, int& key, int& id) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   s = wave_join(s, c2);
   if constexpr (K > 0) {
-    wave_top<K>(top, k, key, id);
-    if (lane < k) { sh.key[wave * k + lane] = key; sh.id[wave * k + lane] = id; }
+    const int n = wave_candidates<K, 16>(top, bar, k, sh.cand + wave * 16);
+    if (lane == 0) sh.count[wave] = n;
   }
   const bool any = __ballot(nan) != 0;
   if (lane == 0) { sh.part[wave] = s; sh.nan[wave] = any; }
@@ -373,10 +437,10 @@ __device__ __forceinline__ bool block_join_row(RowParts<K>& sh, Soft& s, Top<K>&
   for (int w = 1; w < 4; ++w) s.join(sh.part[w], c2);
   nan = sh.nan[0] | sh.nan[1] | sh.nan[2] | sh.nan[3];
   if constexpr (K > 0) {
-    Top<1> one;
-    one.key[0] = lane < 4 * k ? sh.key[lane] : KEY_NONE;
-    one.id[0] = lane < 4 * k ? sh.id[lane] : -1;
-    wave_top<1>(one, k, key, id);
+    int count[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) count[w] = __builtin_amdgcn_readfirstlane(sh.count[w]);
+    first_of<4>((lane & 15) < sh.count[lane >> 4] ? sh.cand[lane] : 0, count, k, sh.sorted, key, id);
   }
   return true;
 }
@@ -409,13 +473,7 @@ __device__ __forceinline__ void enter_above_bar(Top<K>& top, int& bar, const flo
   for (int i = 1; i < N; ++i) most = fmaxf(most, f[i]);
   int mine = odd ? 0x7fffffff : order_key(most);
   if (!__any(mine > bar)) return;
-  int kth = KEY_NONE;
-#pragma unroll
-  for (int j = 0; j < K; ++j) {
-    kth = wave_all(mine, KEY_NONE, Max());
-    if (kth <= bar) break;
-    if ((int)(threadIdx.x & 63) == __ffsll((unsigned long long)__ballot(mine == kth)) - 1) mine = KEY_NONE;
-  }
+  const int kth = kth_largest<K>(mine, bar);
   const float least = key_value(max(kth, bar + 1));
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -429,7 +487,7 @@ template <typename T, int VEC, int K, int WAVES>
 __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, int seg_len, Part* __restrict__ parts,
                                                   int2* __restrict__ part_top) {
   constexpr int UNR = 2, N = VEC * UNR, W = 64 * WAVES;
-  __shared__ RowParts<WAVES == 4 ? K : 0> sh;
+  __shared__ RowParts<K, WAVES> sh[4 / WAVES];
   const int64_t pos = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)
                                  : segments == 1 ? blockIdx.x : blockIdx.x / segments;
   if (WAVES == 1 && pos >= a.positions) return;
@@ -489,10 +547,16 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
   bool nan = nans != 0;
   if constexpr (WAVES == 1) {
     s = wave_join(s, a.c2);
-    if constexpr (K > 0) wave_top<K>(top, a.k, key, id);
+    if constexpr (K > 0) {
+      RowParts<K, WAVES>& mine = sh[threadIdx.x >> 6];
+      const int count[1] = {__builtin_amdgcn_readfirstlane(wave_candidates<K, 64>(top, bar, a.k, mine.cand))};
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      first_of<1>(lane < count[0] ? mine.cand[lane] : 0, count, a.k, mine.sorted, key, id);
+    }
     finish_row(a, pos, l, s, nan, key, id);
   } else {
-    if (!block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) return;
+    if (!block_join_row<K>(sh[0], s, top, bar, nan, a.k, a.c2, key, id)) return;
     if (segments == 1) {
       finish_row(a, pos, l, s, nan, key, id);
       return;
@@ -506,7 +570,7 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
 template <typename T, int K>
 __global__ __launch_bounds__(256) void probs_join(const Args a, int segments, const Part* __restrict__ parts,
                                                   const int2* __restrict__ part_top) {
-  __shared__ RowParts<K> sh;
+  __shared__ RowParts<K, 4> sh;
   const int64_t pos = blockIdx.x;
   Soft s;
   s.clear();
@@ -530,7 +594,9 @@ __global__ __launch_bounds__(256) void probs_join(const Args a, int segments, co
         if (j < a.k && kc[j].y >= 0) top.add(kc[j].x, kc[j].y);
   }
   int key = KEY_NONE, id = -1;
-  if (block_join_row<K>(sh, s, top, nan, a.k, a.c2, key, id)) finish_row(a, pos, l, s, nan, key, id);
+  int bar = KEY_NONE;
+  if constexpr (K > 0) bar = kth_largest<K>(top.key[0], KEY_NONE);
+  if (block_join_row<K>(sh, s, top, bar, nan, a.k, a.c2, key, id)) finish_row(a, pos, l, s, nan, key, id);
 }
 
 // What a thread of probs_planes keeps of the most likely classes of one position: values in falling order.  A new
