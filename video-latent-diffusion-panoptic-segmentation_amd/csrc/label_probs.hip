@@ -210,28 +210,6 @@ __device__ __forceinline__ Soft wave_join(const Soft& s, float c2) {
   return o;
 }
 
-// the n first of the wave's lists, larger key, then lower class: lane j < n gets the j-th
-template <int K>
-__device__ __forceinline__ void wave_top(Top<K>& top, int n, int& key, int& id) {
-  key = KEY_NONE;
-  id = -1;
-  for (int j = 0; j < n; ++j) {
-    const int k = wave_all(top.key[0], KEY_NONE, Max());
-    const bool holds = top.key[0] == k;
-    const unsigned long long who = __ballot(holds);
-    int c = __builtin_amdgcn_readlane(top.id[0], __ffsll(who) - 1);
-    if (who & (who - 1)) c = (int)wave_all(holds ? (unsigned)top.id[0] : ~0u, ~0u, Min());
-    if (c < 0) break;
-    if ((int)(threadIdx.x & 63) == j) { key = k; id = c; }
-    if (holds && top.id[0] == c) {
-#pragma unroll
-      for (int i = 0; i + 1 < K; ++i) { top.key[i] = top.key[i + 1]; top.id[i] = top.id[i + 1]; }
-      top.key[K - 1] = KEY_NONE;
-      top.id[K - 1] = -1;
-    }
-  }
-}
-
 // N adjacent elements at any address aligned to one element: one wide load or store (the card takes unaligned ones)
 template <typename T, int N> struct Pack { T v[N]; };
 template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
@@ -354,80 +332,80 @@ struct Part { float m, r, t; int nan; };
 __device__ __forceinline__ uint64_t candidate(int key, int id) {
   return id < 0 ? 0 : (uint64_t)(uint32_t)(key ^ (int)0x80000000) << 32 | (uint32_t)~id;
 }
-// A wave's share of the candidates for its row's answer, at most CAP of them, written to `to`: the entries of the
-// lanes' lists that are no less than `bar` (which holds the wave's n first), or just those n if there are more.
-template <int K, int CAP>
-__device__ __forceinline__ int wave_candidates(Top<K>& top, int bar, int n, uint64_t* to) {
-  const int lane = threadIdx.x & 63;
-  int count = 0;
-#pragma unroll
-  for (int i = 0; i < K; ++i) {
-    const bool in = top.id[i] >= 0 && top.key[i] >= bar;
-    const uint64_t who = __ballot(in);
-    if (!who) break;
-    const int more = __popcll(who);
-    if (count + more > CAP) {
-      int key, id;
-      wave_top<K>(top, n, key, id);
-      if (lane < n) to[lane] = candidate(key, id);
-      return __popcll(__ballot(lane < n && id >= 0));
-    }
-    if (in) to[count + __popcll(who & ((1ull << lane) - 1))] = candidate(top.key[i], top.id[i]);
-    count += more;
-  }
-  return count;
+__device__ __forceinline__ void wave_lds_fence() {   // a wave's LDS accesses stay in order: only the compiler is held
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
-// The n <= 16 first of a wave's candidates (0: none) in their order, candidates being in runs of `count` at every
-// 64 / RUNS lanes: each finds its place by counting those before it.  Lane j < n gets the j-th.
-template <int RUNS>
-__device__ __forceinline__ void first_of(uint64_t mine, const int (&count)[RUNS], int n, uint64_t* sorted, int& key,
-                                         int& id) {
+// The first n <= 16 of the values that the wave's leading `lanes` lanes hold (0: none), in their order, in every lane
+// j < n: each value finds its place by counting those before it.
+__device__ __forceinline__ uint64_t first_of(uint64_t mine, int lanes, int n, uint64_t* sorted) {
   const int lane = threadIdx.x & 63;
   int place = 0;
-#pragma unroll
-  for (int w = 0; w < RUNS; ++w)
-    for (int j = 0; j < count[w]; ++j) {
-      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), w * (64 / RUNS) + j) << 32 |
-                             (uint32_t)__builtin_amdgcn_readlane((int)mine, w * (64 / RUNS) + j);
-      place += other > mine;
-    }
-  if (lane < 16) sorted[lane] = 0;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  if (mine && place < n) sorted[place] = mine;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  const uint64_t r = lane < n ? sorted[lane] : 0;
-  key = r ? (int)(r >> 32) ^ (int)0x80000000 : KEY_NONE;
-  id = r ? (int)~(uint32_t)r : -1;
-}
-// the K-th largest of the wave's lane values, or what is above none of them
-template <int K> __device__ __forceinline__ int kth_largest(int mine, int floor) {
-  int kth = KEY_NONE;
-#pragma unroll
-  for (int j = 0; j < K; ++j) {
-    kth = wave_all(mine, KEY_NONE, Max());
-    if (kth <= floor) break;
-    if ((int)(threadIdx.x & 63) == __ffsll((unsigned long long)__ballot(mine == kth)) - 1) mine = KEY_NONE;
+  for (int j = 0; j < lanes; ++j) {
+    const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
+    place += other > mine;
   }
-  return kth;
+  if (lane < 16) sorted[lane] = 0;
+  wave_lds_fence();
+  if (mine && place < n) sorted[place] = mine;
+  wave_lds_fence();
+  const uint64_t r = lane < n ? sorted[lane] : 0;
+  wave_lds_fence();
+  return r;
+}
+// What a wave keeps for the answer of its row: candidates in any order, among them the first n of all it was given.
+struct Best {
+  uint64_t some[64], sorted[16];
+};
+__device__ __forceinline__ void absorb(Best& b, int& count, uint64_t mine, int n) {   // a candidate (or 0) a lane
+  const int lane = threadIdx.x & 63;
+  uint64_t who = __ballot(mine != 0);
+  if (count + __popcll(who) > 64) {
+    const uint64_t r = first_of(lane < count ? b.some[lane] : 0, count, n, b.sorted);
+    if (lane < n) b.some[lane] = r;
+    count = __popcll(__ballot(r != 0));
+    if (count + __popcll(who) > 64) {
+      mine = first_of(mine, 64, n, b.sorted);
+      who = __ballot(mine != 0);
+    }
+  }
+  if (mine) b.some[count + __popcll(who & ((1ull << lane) - 1))] = mine;
+  count += __popcll(who);
+  wave_lds_fence();
+}
+// the n-th largest of the wave's lane values, or one that is not above `floor`
+__device__ __forceinline__ int nth_largest(int mine, int n, int floor) {
+  int nth = KEY_NONE;
+  for (int j = 0; j < n; ++j) {
+    nth = wave_all(mine, KEY_NONE, Max());
+    if (nth <= floor) break;
+    if ((int)(threadIdx.x & 63) == __ffsll((unsigned long long)__ballot(mine == nth)) - 1) mine = KEY_NONE;
+  }
+  return nth;
 }
 
-template <int K, int WAVES>
+template <bool TOP, int WAVES>
 struct RowParts {
   Soft part[WAVES];
   int nan[WAVES], count[WAVES];
-  uint64_t cand[K > 0 ? 64 : 1], sorted[K > 0 ? 16 : 1];
+  Best best[TOP ? WAVES : 1];
 };
-// the block's threads' sums and lists joined, in wave 0 (lane j < k: the j-th of the list); other waves get nothing
-template <int K>
-__device__ __forceinline__ bool block_join_row(RowParts<K, 4>& sh, Soft& s, Top<K>& top, int bar, bool& nan, int k,
-                                               float c2, int& key, int& id) {
+// the block's threads' sums and candidates joined, in wave 0 (lane j < n: the j-th of the answer); other waves get
+// nothing
+template <bool TOP>
+__device__ __forceinline__ bool block_join_row(RowParts<TOP, 4>& sh, Soft& s, int count, bool& nan, int n, float c2,
+                                               uint64_t& answer) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   s = wave_join(s, c2);
-  if constexpr (K > 0) {
-    const int n = wave_candidates<K, 16>(top, bar, k, sh.cand + wave * 16);
-    if (lane == 0) sh.count[wave] = n;
+  if constexpr (TOP) {
+    Best& b = sh.best[wave];
+    if (count > 16) {
+      const uint64_t r = first_of(lane < count ? b.some[lane] : 0, count, n, b.sorted);
+      if (lane < n) b.some[lane] = r;
+      count = n;
+    }
+    if (lane == 0) sh.count[wave] = count;
   }
   const bool any = __ballot(nan) != 0;
   if (lane == 0) { sh.part[wave] = s; sh.nan[wave] = any; }
@@ -436,11 +414,11 @@ __device__ __forceinline__ bool block_join_row(RowParts<K, 4>& sh, Soft& s, Top<
   s = sh.part[0];
   for (int w = 1; w < 4; ++w) s.join(sh.part[w], c2);
   nan = sh.nan[0] | sh.nan[1] | sh.nan[2] | sh.nan[3];
-  if constexpr (K > 0) {
-    int count[4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) count[w] = __builtin_amdgcn_readfirstlane(sh.count[w]);
-    first_of<4>((lane & 15) < sh.count[lane >> 4] ? sh.cand[lane] : 0, count, k, sh.sorted, key, id);
+  if constexpr (TOP) {
+    // the waves' candidates side by side: at most 16 of each
+    const int n0 = sh.count[0], n1 = n0 + sh.count[1], n2 = n1 + sh.count[2], all = n2 + sh.count[3];
+    const int w = lane < n0 ? 0 : lane < n1 ? 1 : lane < n2 ? 2 : 3, at = lane - (w == 0 ? 0 : w == 1 ? n0 : w == 2 ? n1 : n2);
+    answer = first_of(lane < all ? sh.best[w].some[at] : 0, __builtin_amdgcn_readfirstlane(all), n, sh.best[0].sorted);
   }
   return true;
 }
@@ -455,39 +433,43 @@ __device__ __forceinline__ LabelAt label_at(const Args& a, int64_t pos) {
     r.xy = to_f(((const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2))[r.y]);
   return r;
 }
-__device__ __forceinline__ void finish_row(const Args& a, int64_t pos, const LabelAt& l, const Soft& s, bool nan, int key,
-                                           int id) {
+__device__ __forceinline__ void finish_row(const Args& a, int64_t pos, const LabelAt& l, const Soft& s, bool nan,
+                                           uint64_t answer) {
   const int lane = threadIdx.x & 63;
   const Result q = result_of(a, s, nan, l.y, l.xy);
   if (lane == 0) store_row(a, pos, s, q);
-  if (lane < a.k) store_top(a, pos, lane, key, id, s, q.ls);
+  if (lane < a.k)
+    store_top(a, pos, lane, (int)(answer >> 32) ^ (int)0x80000000, answer ? (int)~(uint32_t)answer : -1, s, q.ls);
 }
 
-// A turn's classes enter the lanes' lists only above a bar: the K-th largest of the wave's lane maxima, or what an
-// earlier turn had; K classes at least are no less, and later ones lose ties.  So lists see little but the answer.
-template <int K, int N, typename C>
-__device__ __forceinline__ void enter_above_bar(Top<K>& top, int& bar, const float (&f)[N], bool odd, C class_of) {
+// A turn's classes become candidates only above a bar: the n-th largest of the wave's lane maxima, or what an earlier
+// turn had; n classes at least are no less, and later ones lose ties.  So little but the answer is looked at twice.
+template <int N, typename C>
+__device__ __forceinline__ void enter_above_bar(Best& b, int& count, int& bar, int n, const float (&f)[N], bool odd,
+                                                C class_of) {
   if (bar == 0x7fffffff) return;
   float most = f[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) most = fmaxf(most, f[i]);
-  int mine = odd ? 0x7fffffff : order_key(most);
-  if (!__any(mine > bar)) return;
-  const int kth = kth_largest<K>(mine, bar);
-  const float least = key_value(max(kth, bar + 1));
+  const int mine = odd ? 0x7fffffff : order_key(most);
+  const uint64_t over = __ballot(mine > bar);
+  if (!over) return;
+  const int nth = __popcll(over) < n ? bar : nth_largest(mine, n, bar);
+  const float least = key_value(max(nth, bar + 1));
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (__any(!(f[i] < least)))
-      if (!(f[i] < least)) top.add(order_key(f[i]), class_of(i));
-  bar = max(bar, kth);
+  for (int i = 0; i < N; ++i) {
+    const bool in = !(f[i] < least);               // a NaN is
+    if (__any(in)) absorb(b, count, in ? candidate(order_key(f[i]), class_of(i)) : 0, n);
+  }
+  bar = max(bar, nth);
 }
 
 // WAVES = 1: a wave to a row, four rows to a block, for rows that a block's start and end would outweigh.
-template <typename T, int VEC, int K, int WAVES>
+template <typename T, int VEC, bool TOP, int WAVES>
 __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, int seg_len, Part* __restrict__ parts,
-                                                  int2* __restrict__ part_top) {
+                                                  uint64_t* __restrict__ part_top) {
   constexpr int UNR = 2, N = VEC * UNR, W = 64 * WAVES;
-  __shared__ RowParts<K, WAVES> sh[4 / WAVES];
+  __shared__ RowParts<TOP, WAVES> sh[4 / WAVES];
   const int64_t pos = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)
                                  : segments == 1 ? blockIdx.x : blockIdx.x / segments;
   if (WAVES == 1 && pos >= a.positions) return;
@@ -496,22 +478,23 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
   const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
   const uint8_t* mask = a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
   const int end = min(a.classes, (seg + 1) * seg_len), last = a.classes - VEC;
+  RowParts<TOP, WAVES>& mine = sh[WAVES == 1 ? threadIdx.x >> 6 : 0];
+  Best& best = mine.best[TOP && WAVES == 4 ? threadIdx.x >> 6 : 0];
+  int count = 0;                   // the wave's candidates
   Soft s;
   s.clear();
-  Top<K> top;
-  top.clear();
   uint64_t nans = 0;               // lanes that saw one
   LabelAt l;
   if (segments == 1) l = label_at<T>(a, pos);
-  int bar = KEY_NONE;              // the wave's lists hold K keys that are no less
+  int bar = KEY_NONE;              // a.k of them are no less
   auto turn = [&](int at0, float (&f)[N]) {
     uint64_t odd = 0;
 #pragma unroll
     for (int i = 0; i < N; i += 2) odd |= __ballot(__builtin_isunordered(f[i], f[i + 1]));
     nans |= odd;
-    if constexpr (K > 0)
-      enter_above_bar<K, N>(top, bar, f, odd >> lane & 1,
-                            [&](int i) { return min(at0 + i / VEC * W * VEC, last) + i % VEC; });
+    if constexpr (TOP)
+      enter_above_bar<N>(best, count, bar, a.k, f, odd >> lane & 1,
+                         [&](int i) { return min(at0 + i / VEC * W * VEC, last) + i % VEC; });
     s.template add_all<N>(f, a.c2);
   };
   int base = seg * seg_len;        // the same turns in every lane: they exchange values
@@ -543,60 +526,61 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
     }
     turn(at0, f);
   }
-  int key = KEY_NONE, id = -1;
+  uint64_t answer = 0;
   bool nan = nans != 0;
   if constexpr (WAVES == 1) {
     s = wave_join(s, a.c2);
-    if constexpr (K > 0) {
-      RowParts<K, WAVES>& mine = sh[threadIdx.x >> 6];
-      const int count[1] = {__builtin_amdgcn_readfirstlane(wave_candidates<K, 64>(top, bar, a.k, mine.cand))};
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      first_of<1>(lane < count[0] ? mine.cand[lane] : 0, count, a.k, mine.sorted, key, id);
-    }
-    finish_row(a, pos, l, s, nan, key, id);
+    if constexpr (TOP) answer = first_of(lane < count ? best.some[lane] : 0, count, a.k, best.sorted);
+    finish_row(a, pos, l, s, nan, answer);
   } else {
-    if (!block_join_row<K>(sh[0], s, top, bar, nan, a.k, a.c2, key, id)) return;
+    if (!block_join_row<TOP>(mine, s, count, nan, a.k, a.c2, answer)) return;
     if (segments == 1) {
-      finish_row(a, pos, l, s, nan, key, id);
+      finish_row(a, pos, l, s, nan, answer);
       return;
     }
     if (lane == 0) parts[blockIdx.x] = {s.m, s.r, s.t, nan};
-    if (lane < a.k) part_top[(int64_t)blockIdx.x * a.k + lane] = make_int2(key, id);
+    if (lane < a.k) part_top[(int64_t)blockIdx.x * a.k + lane] = answer;
   }
 }
 
-// one block per row: its segments in the order of their classes
-template <typename T, int K>
+// One block per row: its segments' sums and answers joined.
+template <typename T, bool TOP>
 __global__ __launch_bounds__(256) void probs_join(const Args a, int segments, const Part* __restrict__ parts,
-                                                  const int2* __restrict__ part_top) {
-  __shared__ RowParts<K, 4> sh;
+                                                  const uint64_t* __restrict__ part_top) {
+  __shared__ RowParts<TOP, 4> sh;
   const int64_t pos = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  Best& best = sh.best[TOP ? threadIdx.x >> 6 : 0];
   Soft s;
   s.clear();
-  Top<K> top;
-  top.clear();
   bool nan = false;
+  int count = 0, bar = KEY_NONE;
   const LabelAt l = label_at<T>(a, pos);
-  for (int i = threadIdx.x; i < segments; i += 256) {
-    const Part p = parts[pos * segments + i];
-    int2 kc[K > 0 ? K : 1];
+  for (int base = threadIdx.x & ~63; base < segments; base += 256) {   // the same turns in every lane of a wave
+    const int i = base + lane;
+    Part p = {-INFINITY, 0.f, 0.f, 0};
+    uint64_t c[TOP ? 16 : 1];
+    if (i < segments) p = parts[pos * segments + i];
+    if constexpr (TOP)
 #pragma unroll
-    for (int j = 0; j < K; ++j)
-      if (j < a.k) kc[j] = part_top[(pos * segments + i) * a.k + j];
+      for (int j = 0; j < 16; ++j) c[j] = j < a.k && i < segments ? part_top[(pos * segments + i) * a.k + j] : 0;
     Soft o;
     o.m = p.m; o.r = p.r; o.t = p.t;
     s.join(o, a.c2);
     nan |= p.nan != 0;
-    if constexpr (K > 0)
+    if constexpr (TOP) {
+      const int first = c[0] ? (int)(c[0] >> 32) ^ (int)0x80000000 : KEY_NONE;
+      bar = max(bar, nth_largest(first, a.k, bar));
 #pragma unroll
-      for (int j = 0; j < K; ++j)
-        if (j < a.k && kc[j].y >= 0) top.add(kc[j].x, kc[j].y);
+      for (int j = 0; j < 16; ++j) {
+        const bool in = c[j] && ((int)(c[j] >> 32) ^ (int)0x80000000) >= bar;
+        if (!__any(in)) break;                     // each segment's are in falling order
+        absorb(best, count, in ? c[j] : 0, a.k);
+      }
+    }
   }
-  int key = KEY_NONE, id = -1;
-  int bar = KEY_NONE;
-  if constexpr (K > 0) bar = kth_largest<K>(top.key[0], KEY_NONE);
-  if (block_join_row<K>(sh, s, top, bar, nan, a.k, a.c2, key, id)) finish_row(a, pos, l, s, nan, key, id);
+  uint64_t answer = 0;
+  if (block_join_row<TOP>(sh, s, count, nan, a.k, a.c2, answer)) finish_row(a, pos, l, s, nan, answer);
 }
 
 // What a thread of probs_planes keeps of the most likely classes of one position: values in falling order.  A new
@@ -958,21 +942,21 @@ void launch_short(const Args& a, hipStream_t s) {
   if (a.k) hipLaunchKernelGGL((probs_short_rows<T, VEC, G, E, true>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((probs_short_rows<T, VEC, G, E, false>), grid, dim3(256), 0, s, a);
 }
-template <typename T, int K>
-void launch_long_as(const Args& a, int segments, void* ws, hipStream_t s) {
+template <typename T, bool TOP>
+void launch_long(const Args& a, int segments, void* ws, hipStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   if (a.positions >= 2048 && a.classes <= WAVE_CLASSES) {
-    hipLaunchKernelGGL((probs_rows<T, VEC, K, 1>), dim3((unsigned)((a.positions + 3) / 4)), dim3(256), 0, s, a, 1,
-                       a.classes, (Part*)nullptr, (int2*)nullptr);
+    hipLaunchKernelGGL((probs_rows<T, VEC, TOP, 1>), dim3((unsigned)((a.positions + 3) / 4)), dim3(256), 0, s, a, 1,
+                       a.classes, (Part*)nullptr, (uint64_t*)nullptr);
     return;
   }
   const int reach = 256 * VEC, per = ((a.classes + reach - 1) / reach + segments - 1) / segments;
   Part* parts = (Part*)ws;
-  int2* tops = (int2*)(parts + a.positions * segments);
-  hipLaunchKernelGGL((probs_rows<T, VEC, K, 4>), dim3((unsigned)(a.positions * segments)), dim3(256), 0, s, a, segments,
-                     per * reach, parts, tops);
+  uint64_t* tops = (uint64_t*)(parts + a.positions * segments);
+  hipLaunchKernelGGL((probs_rows<T, VEC, TOP, 4>), dim3((unsigned)(a.positions * segments)), dim3(256), 0, s, a,
+                     segments, per * reach, parts, tops);
   if (segments > 1)
-    hipLaunchKernelGGL((probs_join<T, K>), dim3((unsigned)a.positions), dim3(256), 0, s, a, segments, parts, tops);
+    hipLaunchKernelGGL((probs_join<T, TOP>), dim3((unsigned)a.positions), dim3(256), 0, s, a, segments, parts, tops);
 }
 
 template <typename T>
@@ -981,11 +965,8 @@ int launch(const Args& a, void* ws, hipStream_t s) {
   if (a.sc == 1 && a.classes > SHORT_CLASSES) {
     const int segments = segments_of(a.positions, a.classes, sizeof(T) == 2 ? LDM_BF16 : LDM_F32);
     if ((a.classes <= WAVE_CLASSES ? (a.positions + 3) / 4 : a.positions * segments) > MOST_BLOCKS) return LDM_ERR_ARG;
-    if (a.k == 0) launch_long_as<T, 0>(a, segments, ws, s);
-    else if (a.k == 1) launch_long_as<T, 1>(a, segments, ws, s);
-    else if (a.k <= 4) launch_long_as<T, 4>(a, segments, ws, s);
-    else if (a.k <= 8) launch_long_as<T, 8>(a, segments, ws, s);
-    else launch_long_as<T, 16>(a, segments, ws, s);
+    if (a.k) launch_long<T, true>(a, segments, ws, s);
+    else launch_long<T, false>(a, segments, ws, s);
   } else if (a.sc == 1 && a.classes >= VEC) {
     const int lanes = (a.classes + 15) / 16;
     if ((a.positions * lanes + 127) / 128 > MOST_BLOCKS) return LDM_ERR_ARG;      // lanes round up to a power of two
@@ -1055,7 +1036,7 @@ extern "C" size_t ldm_label_log_probs_workspace_bytes(const ldm_label_probs_para
   if (!p || !long_rows(p) || p->n0 <= 0 || p->n1 <= 0 || p->n2 <= 0) return 0;
   const int64_t n = p->n0 * p->n1 * p->n2;
   const int segments = segments_of(n, p->classes, p->dtype);
-  return segments == 1 ? 0 : (size_t)(n * segments) * (sizeof(Part) + sizeof(int2) * (size_t)std::max(0, p->topk));
+  return segments == 1 ? 0 : (size_t)(n * segments) * (sizeof(Part) + sizeof(uint64_t) * (size_t)std::max(0, p->topk));
 }
 
 extern "C" int ldm_label_log_probs(const ldm_label_probs_params* p, ldm_stream_t stream) {
