@@ -25,7 +25,7 @@ constexpr float LOWEST = -3e38f;   // finite stand-in for x_j - m = -inf: 0 * LO
 
 struct Args {
   const void* x;
-  int64_t n1, n2, s0, s1, s2, sc, positions;
+  int64_t n1, n2, s0, s1, s2, sc, positions;       // n1 = 0: all positions are in the last dim
   int classes;
   const int64_t* labels;
   int64_t ignore;
@@ -38,6 +38,11 @@ struct Args {
   int k;
 };
 
+// a / b, a < all: in 32 bits where all and b fit, which every thread of a launch decides alike
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b, int64_t all) {
+  if ((uint64_t)(all | b) >> 32 == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+  return a / b;
+}
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // order-preserving float -> int32 with NaN above everything and -0 equal to +0
@@ -157,14 +162,20 @@ __device__ __forceinline__ Result result_of(const Args& a, const Soft& s, bool n
   return q;
 }
 __device__ __forceinline__ void store_top(const Args& a, int64_t pos, int j, int key, int id, const Soft& s, float ls) {
-  const int64_t o = pos / a.inner, at = (o * a.k + j) * a.inner + (pos - o * a.inner);
+  const int64_t o = a.inner == 1 ? pos : quotient(pos, a.inner, a.positions), at = (o * a.k + j) * a.inner + (pos - o * a.inner);
   a.top_id[at] = id;
   a.top_lp[at] = id < 0 ? -INFINITY : (key_value(key) - s.m) * a.inv_t - ls;
 }
 
-__device__ __forceinline__ int64_t offset_of(int64_t pos, int64_t n1, int64_t n2, int64_t s0, int64_t s1, int64_t s2) {
-  const int64_t line = pos / n2;
-  return (line / n1) * s0 + (line % n1) * s1 + (pos % n2) * s2;
+// a position's three indices
+struct Place {
+  int64_t i0, i1, i2;
+  __device__ __forceinline__ int64_t at(int64_t s0, int64_t s1, int64_t s2) const { return i0 * s0 + i1 * s1 + i2 * s2; }
+};
+__device__ __forceinline__ Place place_of(int64_t pos, int64_t all, int64_t n1, int64_t n2) {
+  if (n1 == 0) return {0, 0, pos};                 // all positions in one dim
+  const int64_t line = quotient(pos, n2, all), i0 = n1 == 1 ? line : quotient(line, n1, all);
+  return {i0, line - i0 * n1, pos - line * n2};
 }
 
 // Reductions by DPP, in the vector pipe; a shuffle is a trip through LDS.
@@ -251,8 +262,8 @@ __global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
   const int64_t want = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
   const bool live = want < a.positions;
   const int64_t pos = live ? want : a.positions - 1;
-  const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
-  const uint8_t* mask = a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
+  const T* x = (const T*)a.x + place_of(pos, a.positions, a.n1, a.n2).at(a.s0, a.s1, a.s2);
+  const uint8_t* mask = a.mask ? a.mask + quotient(pos, a.mask_div, a.positions) * a.mask_stride : nullptr;
   Pack<T, VEC> v[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = load_pack<T, VEC>(x + min((sub + e * G) * VEC, a.classes - VEC));
@@ -429,8 +440,8 @@ __device__ __forceinline__ LabelAt label_at(const Args& a, int64_t pos) {
   LabelAt r = {-1, -INFINITY};
   if (!a.labels) return r;
   r.y = a.labels[pos];
-  if (r.y >= 0 && r.y < a.classes && !(a.mask && !a.mask[(pos / a.mask_div) * a.mask_stride + r.y]))
-    r.xy = to_f(((const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2))[r.y]);
+  if (r.y >= 0 && r.y < a.classes && !(a.mask && !a.mask[quotient(pos, a.mask_div, a.positions) * a.mask_stride + r.y]))
+    r.xy = to_f(((const T*)a.x + place_of(pos, a.positions, a.n1, a.n2).at(a.s0, a.s1, a.s2))[r.y]);
   return r;
 }
 __device__ __forceinline__ void finish_row(const Args& a, int64_t pos, const LabelAt& l, const Soft& s, bool nan,
@@ -475,8 +486,8 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
   if (WAVES == 1 && pos >= a.positions) return;
   const int seg = segments == 1 ? 0 : (int)(blockIdx.x - pos * segments);
   const int tid = threadIdx.x & (W - 1), lane = tid & 63;
-  const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
-  const uint8_t* mask = a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
+  const T* x = (const T*)a.x + place_of(pos, a.positions, a.n1, a.n2).at(a.s0, a.s1, a.s2);
+  const uint8_t* mask = a.mask ? a.mask + quotient(pos, a.mask_div, a.positions) * a.mask_stride : nullptr;
   const int end = min(a.classes, (seg + 1) * seg_len), last = a.classes - VEC;
   RowParts<TOP, WAVES>& mine = sh[WAVES == 1 ? threadIdx.x >> 6 : 0];
   Best& best = mine.best[TOP && WAVES == 4 ? threadIdx.x >> 6 : 0];
@@ -657,8 +668,8 @@ __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling t
   if (LISTED) n = list_classes(a.mask + row * a.mask_stride, a.classes, list);
   if (!SPLIT && !live) return;
   const int64_t pos = live ? row * tile.run + want : a.positions - 1;
-  const T* x = (const T*)a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
-  const uint8_t* mask = a.mask ? a.mask + (LISTED ? row : pos / a.mask_div) * a.mask_stride : nullptr;
+  const T* x = (const T*)a.x + place_of(pos, a.positions, a.n1, a.n2).at(a.s0, a.s1, a.s2);
+  const uint8_t* mask = a.mask ? a.mask + (LISTED ? row : quotient(pos, a.mask_div, a.positions)) * a.mask_stride : nullptr;
   const int c0 = SPLIT ? (int)((int64_t)n * wave >> 2) : 0;
   const int c1 = SPLIT ? (int)((int64_t)n * (wave + 1) >> 2) : n;
   int64_t y = -1;
@@ -734,7 +745,7 @@ __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling t
   const Result q = result_of(a, s, nan, y, xy);
   store_row(a, pos, s, q);
   if constexpr (K > 0) {
-    const int64_t o = a.inner == 1 ? pos : pos / a.inner, at = o * a.k * a.inner + pos - o * a.inner;
+    const int64_t o = a.inner == 1 ? pos : quotient(pos, a.inner, a.positions), at = o * a.k * a.inner + pos - o * a.inner;
     if (nan) {
       // every value is NaN: the classes that are come first, lower class first, then the others by value
       Top<K> keys;
@@ -804,9 +815,10 @@ __global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, cons
   }
   const int64_t pos = row * tile.run + want;
   if (want >= tile.run || pos >= a.positions) return;
-  const T* x = a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
-  T* dx = a.dx + offset_of(pos, a.n1, a.n2, a.o0, a.o1, a.o2);
-  const uint8_t* mask = !UNIFORM && a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
+  const Place place = place_of(pos, a.positions, a.n1, a.n2);
+  const T* x = a.x + place.at(a.s0, a.s1, a.s2);
+  T* dx = a.dx + place.at(a.o0, a.o1, a.o2);
+  const uint8_t* mask = !UNIFORM && a.mask ? a.mask + quotient(pos, a.mask_div, a.positions) * a.mask_stride : nullptr;
   T v[UNR];
   auto load = [&](int c) {
 #pragma unroll
@@ -844,9 +856,10 @@ __global__ __launch_bounds__(256) void probs_bwd_rows(const BwdArgs<T> a, unsign
     pos = blockIdx.x / blocks_per_row;
     first = (blockIdx.x - (unsigned)pos * blocks_per_row) * (256 * UN) + threadIdx.x;
   }
-  const T* x = a.x + offset_of(pos, a.n1, a.n2, a.s0, a.s1, a.s2);
-  T* dx = a.dx + offset_of(pos, a.n1, a.n2, a.o0, a.o1, a.o2);
-  const uint8_t* mask = a.mask ? a.mask + (pos / a.mask_div) * a.mask_stride : nullptr;
+  const Place place = place_of(pos, a.positions, a.n1, a.n2);
+  const T* x = a.x + place.at(a.s0, a.s1, a.s2);
+  T* dx = a.dx + place.at(a.o0, a.o1, a.o2);
+  const uint8_t* mask = a.mask ? a.mask + quotient(pos, a.mask_div, a.positions) * a.mask_stride : nullptr;
   Pack<T, VEC> v[UN];
 #pragma unroll
   for (int u = 0; u < UN; ++u) {
@@ -988,7 +1001,7 @@ template <typename T>
 int launch_bwd(const ldm_label_probs_bwd_params* p, int64_t n, hipStream_t s) {
   BwdArgs<T> a;
   a.x = (const T*)p->logits; a.dx = (T*)p->d_logits;
-  a.n1 = p->n1; a.n2 = p->n2;
+  a.n1 = n == p->n2 ? 0 : p->n1; a.n2 = p->n2;
   a.s0 = p->s0; a.s1 = p->s1; a.s2 = p->s2; a.sc = p->sc;
   a.o0 = p->o0; a.o1 = p->o1; a.o2 = p->o2; a.oc = p->oc;
   a.positions = n; a.classes = (int)p->classes;
@@ -1053,7 +1066,7 @@ extern "C" int ldm_label_log_probs(const ldm_label_probs_params* p, ldm_stream_t
   if (need && (!p->workspace || p->workspace_bytes < need)) return LDM_ERR_ARG;
   Args a;
   a.x = p->logits;
-  a.n1 = p->n1; a.n2 = p->n2; a.s0 = p->s0; a.s1 = p->s1; a.s2 = p->s2; a.sc = p->sc;
+  a.n1 = n == p->n2 ? 0 : p->n1; a.n2 = p->n2; a.s0 = p->s0; a.s1 = p->s1; a.s2 = p->s2; a.sc = p->sc;
   a.positions = n; a.classes = (int)p->classes;
   a.labels = p->labels; a.ignore = p->ignore_label; a.has_ignore = p->has_ignore;
   a.mask = (const uint8_t*)p->class_mask; a.mask_stride = p->mask_stride; a.mask_div = p->mask_div;
