@@ -481,7 +481,8 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
                                                   uint64_t* __restrict__ part_top) {
   constexpr int UNR = 2, N = VEC * UNR, W = 64 * WAVES;
   __shared__ RowParts<TOP, WAVES> sh[4 / WAVES];
-  const int64_t pos = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);     // a scalar, and so is the row's address
+  const int64_t pos = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave
                                  : segments == 1 ? blockIdx.x : blockIdx.x / segments;
   if (WAVES == 1 && pos >= a.positions) return;
   const int seg = segments == 1 ? 0 : (int)(blockIdx.x - pos * segments);
@@ -489,8 +490,8 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
   const T* x = (const T*)a.x + place_of(pos, a.positions, a.n1, a.n2).at(a.s0, a.s1, a.s2);
   const uint8_t* mask = a.mask ? a.mask + quotient(pos, a.mask_div, a.positions) * a.mask_stride : nullptr;
   const int end = min(a.classes, (seg + 1) * seg_len), last = a.classes - VEC;
-  RowParts<TOP, WAVES>& mine = sh[WAVES == 1 ? threadIdx.x >> 6 : 0];
-  Best& best = mine.best[TOP && WAVES == 4 ? threadIdx.x >> 6 : 0];
+  RowParts<TOP, WAVES>& mine = sh[WAVES == 1 ? wave : 0];
+  Best& best = mine.best[TOP && WAVES == 4 ? wave : 0];
   int count = 0;                   // the wave's candidates
   Soft s;
   s.clear();
