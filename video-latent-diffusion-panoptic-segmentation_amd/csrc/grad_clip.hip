@@ -17,22 +17,28 @@
 namespace {
 
 constexpr int TABLE = 224;               // spans to a launch: 16 B each, below the 4 KB of kernel arguments
-constexpr int PACKS = 8;                 // 16-byte packs of a chunk to a thread, all in flight: 32 KB to a block
+// A chunk is a block's: PACKS packs of 16 bytes to a thread, all in flight.  8 of them (32 KB) carry the most bytes a
+// second; a call of less than SMALL_BYTES takes 2, for more blocks (1.2 MB: 8.5 us, 10.2 us with 8).
+constexpr int LARGE_PACKS = 8, SMALL_PACKS = 2;
+constexpr int64_t SMALL_BYTES = 8 << 20;
 constexpr int MAX_BLOCKS = 2048;
+constexpr int JOIN_CHUNKS = 1024;        // up to here a launch costs more than every block's own join of the partials
 
 template <typename T> struct Pack { T v[16 / sizeof(T)]; };
-template <typename T> constexpr int chunk_of() { return 256 * PACKS * 16 / (int)sizeof(T); }
+constexpr int chunk_bytes(int packs) { return 256 * 16 * packs; }
+template <typename T, int PACKS> constexpr int chunk_of() { return chunk_bytes(PACKS) / (int)sizeof(T); }
 
 struct Entry {
   uint64_t ptr;                          // bit 63: bf16
   uint32_t n, chunk0;                    // elements, first chunk
 };
-struct Table {
+template <int P> struct Table {
+  static constexpr int packs = P;
   Entry e[TABLE];
   int count, chunks;
 };
 
-__device__ __forceinline__ int entry_of(const Table& t, int chunk) {   // the last entry with chunk0 <= chunk
+template <int P> __device__ __forceinline__ int entry_of(const Table<P>& t, int chunk) {   // the last entry with chunk0 <= chunk
   int lo = 0, hi = t.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -66,11 +72,11 @@ template <int NORM, int WAVES = 4> __device__ __forceinline__ double block_join(
 // A thread's packs of a chunk's elements [0, n), at any address aligned to one element: all loads in flight, then
 // ready() (false: nothing more), pack(index, pack) for each whole one and rest(element, value) for an element behind
 // the last.
-template <typename T, typename Q, typename P, typename R>
+template <int PACKS, typename T, typename Q, typename P, typename R>
 __device__ __forceinline__ void each_pack(const T* g, int n, Q ready, P pack, R rest) {
   constexpr int V = 16 / (int)sizeof(T);
   Pack<T> p[PACKS];
-  if (n == chunk_of<T>()) {
+  if (n == chunk_of<T, PACKS>()) {
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) __builtin_memcpy(&p[i], g + (i * 256 + threadIdx.x) * V, 16);
     if (!ready()) return;
@@ -91,9 +97,9 @@ __device__ __forceinline__ void each_pack(const T* g, int n, Q ready, P pack, R 
     if (i * 256 + (int)threadIdx.x < whole) pack(i * 256 + (int)threadIdx.x, p[i]);
 }
 
-template <int NORM, typename T>
+template <int NORM, int PACKS, typename T>
 __device__ __forceinline__ double chunk_norm(const T* g, int n, double acc) {
-  each_pack(g, n, [] { return true; }, [&](int, const Pack<T>& p) {
+  each_pack<PACKS>(g, n, [] { return true; }, [&](int, const Pack<T>& p) {
 #pragma unroll
     for (int j = 0; j < 16 / (int)sizeof(T); ++j) acc = norm_add<NORM>(acc, to_f(p.v[j]));
   }, [&](int, T v) { acc = norm_add<NORM>(acc, to_f(v)); });
@@ -106,18 +112,19 @@ struct Chunk {
   uint64_t ptr;                          // bit 63: bf16
   int n;
 };
-struct ChunkList {
+template <int P> struct ChunkList {
+  static constexpr int packs = P;
   const Chunk* at;
   int chunks;
 };
-__device__ __forceinline__ Chunk chunk_at(const ChunkList& l, int c) { return l.at[c]; }
-__device__ __forceinline__ Chunk chunk_of_entry(const Entry& e, int k) {
-  const int64_t len = e.ptr >> 63 ? chunk_of<bf16_t>() : chunk_of<float>(), at = k * len;
-  return {e.ptr + (uint64_t)k * (256 * PACKS * 16), (int)min(len, (int64_t)e.n - at)};
+template <int P> __device__ __forceinline__ Chunk chunk_at(const ChunkList<P>& l, int c) { return l.at[c]; }
+template <int P> __device__ __forceinline__ Chunk chunk_of_entry(const Entry& e, int k) {
+  const int64_t len = e.ptr >> 63 ? chunk_of<bf16_t, P>() : chunk_of<float, P>(), at = k * len;
+  return {e.ptr + (uint64_t)k * chunk_bytes(P), (int)min(len, (int64_t)e.n - at)};
 }
-__device__ __forceinline__ Chunk chunk_at(const Table& t, int c) {
+template <int P> __device__ __forceinline__ Chunk chunk_at(const Table<P>& t, int c) {
   const Entry e = t.e[entry_of(t, c)];
-  return chunk_of_entry(e, c - (int)e.chunk0);
+  return chunk_of_entry<P>(e, c - (int)e.chunk0);
 }
 template <typename S, typename F> __device__ __forceinline__ void with_chunk(const S& s, int c, F f) {
   const Chunk k = chunk_at(s, c);
@@ -126,17 +133,18 @@ template <typename S, typename F> __device__ __forceinline__ void with_chunk(con
 }
 
 // a table's chunks, a block for each span
-__global__ __launch_bounds__(64) void list_chunks(const Table t, Chunk* __restrict__ to) {
+template <int P>
+__global__ __launch_bounds__(64) void list_chunks(const Table<P> t, Chunk* __restrict__ to) {
   const Entry e = t.e[blockIdx.x];
   const int n = (blockIdx.x + 1 < (unsigned)t.count ? (int)t.e[blockIdx.x + 1].chunk0 : t.chunks) - (int)e.chunk0;
-  for (int k = threadIdx.x; k < n; k += 64) to[(int)e.chunk0 + k] = chunk_of_entry(e, k);
+  for (int k = threadIdx.x; k < n; k += 64) to[(int)e.chunk0 + k] = chunk_of_entry<P>(e, k);
 }
 
 template <int NORM, typename S>
 __global__ __launch_bounds__(256) void norm_parts(const S t, double* __restrict__ part) {
   double acc = 0.0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x)
-    with_chunk(t, c, [&](const auto* g, int n) { acc = chunk_norm<NORM>(g, n, acc); });
+    with_chunk(t, c, [&](const auto* g, int n) { acc = chunk_norm<NORM, S::packs>(g, n, acc); });
   acc = block_join<NORM>(acc);
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
 }
@@ -147,11 +155,9 @@ __device__ __forceinline__ float factor_of(float norm, float max_norm) {
   return f > 1.f ? 1.f : f;
 }
 
-// the partials joined: the norm and the factor, in every thread of the block
+// the threads' sums joined: the norm and the factor, in every thread of the block
 template <int NORM>
-__device__ __forceinline__ float2 norm_of(const double* __restrict__ part, int parts, float max_norm) {
-  double acc = 0.0;
-  for (int i = threadIdx.x; i < parts; i += 256) acc = norm_join<NORM>(acc, part[i]);
+__device__ __forceinline__ float2 norm_of(double acc, float max_norm) {
   acc = block_join<NORM>(acc);
   const float norm = (float)(NORM == LDM_NORM_2 ? sqrt(acc) : acc);
   return make_float2(norm, factor_of(norm, max_norm));
@@ -160,17 +166,19 @@ __device__ __forceinline__ float2 norm_of(const double* __restrict__ part, int p
 template <int NORM>
 __global__ __launch_bounds__(256) void norm_final(const double* __restrict__ part, int parts, float max_norm,
                                                   float* __restrict__ out) {
-  const float2 r = norm_of<NORM>(part, parts, max_norm);
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < parts; i += 256) acc = norm_join<NORM>(acc, part[i]);
+  const float2 r = norm_of<NORM>(acc, max_norm);
   if (threadIdx.x == 0) { out[0] = r.x; out[1] = r.y; }
 }
 
 // a gradient is multiplied by the factor as its own type holds it and rounded once, as torch's in-place product
 // of a tensor with a device scalar is: a bf16 gradient's factor has 8 bits
-template <typename T, typename F>
+template <int PACKS, typename T, typename F>
 __device__ __forceinline__ void chunk_scale(T* g, int n, F factor) {
   constexpr int V = 16 / (int)sizeof(T);
   float f;
-  each_pack(g, n, [&] { f = to_f(from_f<T>(factor())); return f != 1.f; }, [&](int i, Pack<T> p) {
+  each_pack<PACKS>(g, n, [&] { f = to_f(from_f<T>(factor())); return f != 1.f; }, [&](int i, Pack<T> p) {
 #pragma unroll
     for (int j = 0; j < V; ++j) p.v[j] = from_f<T>(to_f(p.v[j]) * f);
     __builtin_memcpy(g + i * V, &p, 16);
@@ -184,19 +192,28 @@ __global__ __launch_bounds__(256) void scale_all(const S t, const float* __restr
   const float f = out[1];
   if (f == 1.f) return;
   for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x)
-    with_chunk(t, c, [&](auto* g, int n) { chunk_scale(g, n, [&] { return f; }); });
+    with_chunk(t, c, [&](auto* g, int n) { chunk_scale<S::packs>(g, n, [&] { return f; }); });
 }
 // the same where partials are few: every block joins them itself, beside its first chunk's loads, which takes a
 // launch less
 template <int NORM, typename S>
 __global__ __launch_bounds__(256) void scale_joined(const S t, const double* __restrict__ part, int parts,
                                                     float max_norm, float* __restrict__ out) {
+  double p[JOIN_CHUNKS / 256];
+#pragma unroll
+  for (int j = 0; j < JOIN_CHUNKS / 256; ++j) {
+    const int i = j * 256 + (int)threadIdx.x;
+    p[j] = i < parts ? part[i] : 0.0;              // 0 adds nothing to any of the norms
+  }
   float f = -1.f;
   for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0 && f != 1.f; c -= gridDim.x)
     with_chunk(t, c, [&](auto* g, int n) {
-      chunk_scale(g, n, [&] {
+      chunk_scale<S::packs>(g, n, [&] {
         if (f == -1.f) {
-          const float2 r = norm_of<NORM>(part, parts, max_norm);
+          double acc = p[0];
+#pragma unroll
+          for (int j = 1; j < JOIN_CHUNKS / 256; ++j) acc = norm_join<NORM>(acc, p[j]);
+          const float2 r = norm_of<NORM>(acc, max_norm);
           if (blockIdx.x == 0 && threadIdx.x == 0) { out[0] = r.x; out[1] = r.y; }
           f = r.y;
         }
@@ -288,8 +305,6 @@ int64_t entries_of(const int64_t* numel, int n) {
   return c;
 }
 
-constexpr int JOIN_CHUNKS = 1024;        // a pass of few chunks: a launch costs more than every block's own join
-
 template <int NORM, typename S>
 int launch(const S& t, float max_norm, int clip, float* out, double* part, hipStream_t s) {
   const dim3 grid(std::max(1, std::min(t.chunks, MAX_BLOCKS))), block(256);
@@ -328,15 +343,57 @@ int launch_small(const SmallTable& t, int norm_type, float max_norm, int clip, f
 
 }  // namespace
 
-// partials, and behind them the chunk list where there may be more spans than a table holds (a span has one chunk
-// more than its whole ones at most, and a bf16 chunk has twice the elements)
+// partials, and behind them the chunk list where there may be more spans than a table holds: no more chunks than
+// fp32 ones of the size that the call may take
 extern "C" size_t ldm_grad_norm_workspace_bytes(const int64_t* numel, int ntensors) {
   if (!numel || ntensors <= 0) return 0;
-  size_t chunks = 0;
+  int64_t total = 0, small = 0, large = 0;
   for (int i = 0; i < ntensors; ++i)
-    if (numel[i] > 0) chunks += (size_t)((numel[i] + chunk_of<float>() - 1) / chunk_of<float>());
-  return MAX_BLOCKS * sizeof(double) + (entries_of(numel, ntensors) > TABLE ? chunks * sizeof(Chunk) : 0);
+    if (numel[i] > 0) {
+      total += numel[i];
+      small += (numel[i] + chunk_of<float, SMALL_PACKS>() - 1) / chunk_of<float, SMALL_PACKS>();
+      large += (numel[i] + chunk_of<float, LARGE_PACKS>() - 1) / chunk_of<float, LARGE_PACKS>();
+    }
+  const int64_t chunks = total * 2 < SMALL_BYTES ? small : large;       // 2 bytes an element at least
+  return MAX_BLOCKS * sizeof(double) + (entries_of(numel, ntensors) > TABLE ? (size_t)chunks * sizeof(Chunk) : 0);
 }
+
+namespace {
+struct Span { uint64_t lo, hi, size; };
+
+// spans laid out in tables, and the launches
+template <int P>
+int run(const std::vector<Span>& spans, int norm_type, float max_norm, int clip, float* out, double* part, hipStream_t s) {
+  std::vector<Table<P>> tables(1);
+  tables[0].count = tables[0].chunks = 0;
+  int64_t chunks = 0;
+  for (const Span& p : spans) {
+    const int64_t total = (int64_t)((p.hi - p.lo) / p.size);
+    for (int64_t at = 0; at < total; at += PIECE) {
+      if (tables.back().count == TABLE) {
+        tables.emplace_back();
+        tables.back().count = tables.back().chunks = 0;
+      }
+      Table<P>& t = tables.back();
+      const int64_t n = std::min(PIECE, total - at);
+      t.e[t.count++] = {(p.lo + p.size * (uint64_t)at) | ((uint64_t)(p.size == 2) << 63), (uint32_t)n, (uint32_t)t.chunks};
+      const int more = (int)((n * (int64_t)p.size + chunk_bytes(P) - 1) / chunk_bytes(P));
+      t.chunks += more;
+      chunks += more;
+    }
+  }
+  if (tables.size() == 1) return launch(tables[0], norm_type, max_norm, clip, out, part, s);
+  if (chunks > 0x7fffffff) return LDM_ERR_ARG;
+  Chunk* list = reinterpret_cast<Chunk*>(part + MAX_BLOCKS);
+  chunks = 0;
+  for (const Table<P>& t : tables) {
+    hipLaunchKernelGGL((list_chunks<P>), dim3(t.count), dim3(64), 0, s, t, list + chunks);
+    LDM_CHECK_LAUNCH();
+    chunks += t.chunks;
+  }
+  return launch(ChunkList<P>{list, (int)chunks}, norm_type, max_norm, clip, out, part, s);
+}
+}  // namespace
 
 extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, const uint8_t* dtypes, int ntensors,
                              int norm_type, double max_norm, int clip, float* out, void* workspace,
@@ -345,10 +402,10 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
   if (norm_type < LDM_NORM_2 || norm_type > LDM_NORM_1 || !(max_norm >= 0.0)) return LDM_ERR_ARG;
   if (!workspace || workspace_bytes < (int64_t)ldm_grad_norm_workspace_bytes(numel, ntensors)) return LDM_ERR_ARG;
   // Tensors in the order of their addresses; those that lie back to back (views of a bucket) are one span.
-  struct Span { uint64_t lo, hi, size; };
-  std::vector<Span> spans;
-  std::vector<Table> tables;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  double* part = static_cast<double*>(workspace);
   try {
+    std::vector<Span> spans;
     spans.reserve(ntensors);
     for (int i = 0; i < ntensors; ++i) {
       if (numel[i] < 0 || dtypes[i] > LDM_BF16) return LDM_ERR_ARG;
@@ -367,8 +424,11 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
       else spans[++last] = spans[i];
     }
     if (!spans.empty()) spans.resize(last + 1);
-    int64_t units = 0;
-    for (const Span& p : spans) units += (int64_t)(p.hi - p.lo + 1023) / 1024;
+    int64_t units = 0, bytes = 0;
+    for (const Span& p : spans) {
+      bytes += (int64_t)(p.hi - p.lo);
+      units += (int64_t)(p.hi - p.lo + 1023) / 1024;
+    }
     if (clip != 2 && units <= UNITS * SMALL_WAVES && spans.size() <= SMALL_SPANS) {
       SmallTable t;
       t.units = 0;
@@ -377,44 +437,11 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
         t.e[i] = {p.lo | ((uint64_t)(p.size == 2) << 63), (uint32_t)((p.hi - p.lo) / p.size), (uint32_t)t.units};
         for (int64_t k = (int64_t)(p.hi - p.lo + 1023) / 1024; k > 0; --k) t.span[t.units++] = (uint8_t)i;
       }
-      return launch_small(t, norm_type, (float)max_norm, clip, out, reinterpret_cast<hipStream_t>(stream));
+      return launch_small(t, norm_type, (float)max_norm, clip, out, s);
     }
-    for (const Span& p : spans) {
-      const int64_t total = (int64_t)((p.hi - p.lo) / p.size);
-      const int64_t chunk = p.size == 2 ? chunk_of<bf16_t>() : chunk_of<float>();
-      for (int64_t at = 0; at < total; at += PIECE) {
-        if (tables.empty() || tables.back().count == TABLE) {
-          tables.emplace_back();
-          tables.back().count = tables.back().chunks = 0;
-        }
-        Table& t = tables.back();
-        const int64_t n = std::min(PIECE, total - at);
-        t.e[t.count++] = {(p.lo + p.size * (uint64_t)at) | ((uint64_t)(p.size == 2) << 63), (uint32_t)n,
-                          (uint32_t)t.chunks};
-        t.chunks += (int)((n + chunk - 1) / chunk);
-      }
-    }
-  } catch (...) {
+    return bytes < SMALL_BYTES ? run<SMALL_PACKS>(spans, norm_type, (float)max_norm, clip, out, part, s)
+                               : run<LARGE_PACKS>(spans, norm_type, (float)max_norm, clip, out, part, s);
+  } catch (...) {                  // no exception leaves a C entry; std::bad_alloc is the only one
     return LDM_ERR_ARG;
   }
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  double* part = static_cast<double*>(workspace);
-  if (tables.size() <= 1) {
-    if (tables.empty()) {
-      tables.emplace_back();
-      tables[0].count = tables[0].chunks = 0;
-    }
-    return launch(tables[0], norm_type, (float)max_norm, clip, out, part, s);
-  }
-  Chunk* list = reinterpret_cast<Chunk*>(part + MAX_BLOCKS);
-  int64_t chunks = 0;
-  for (const Table& t : tables) chunks += t.chunks;
-  if (chunks > 0x7fffffff) return LDM_ERR_ARG;
-  chunks = 0;
-  for (const Table& t : tables) {
-    hipLaunchKernelGGL(list_chunks, dim3(t.count), dim3(64), 0, s, t, list + chunks);
-    LDM_CHECK_LAUNCH();
-    chunks += t.chunks;
-  }
-  return launch(ChunkList{list, (int)chunks}, norm_type, (float)max_norm, clip, out, part, s);
 }
