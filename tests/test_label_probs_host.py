@@ -82,7 +82,8 @@ def test_c_entries_refuse_before_any_launch():
         p = K.LabelProbsBwdParams(**{**okb, **bad})
         assert lib.ldm_label_log_probs_bwd(ctypes.byref(p), None) == 1, bad
     u64, i64 = ctypes.c_uint64, ctypes.c_int64
-    ptrs, numel = (u64 * 2)(4096, 8192), (i64 * 2)(16, 16)
+    ptrs, numel = (u64 * 2)(4096, 1 << 20), (i64 * 2)(16, 65536)
+    assert lib.ldm_grad_norm_workspace_bytes((i64 * 2)(16, 16), 2) == 0      # one block takes no partials
     wsb = lib.ldm_grad_norm_workspace_bytes(numel, 2)
     assert wsb > 0
 
@@ -91,13 +92,13 @@ def test_c_entries_refuse_before_any_launch():
 
     assert norm(ptrs=(u64 * 2)(4096, 4096)) == norm(ptrs=(u64 * 2)(4096, 4156)) == ERR_OVERLAP
     assert "overlap" in lib.ldm_status_string(ERR_OVERLAP).decode()
-    for kw in (dict(ptrs=(u64 * 2)(0, 8192)),
+    for kw in (dict(ptrs=(u64 * 2)(0, 1 << 20)),
                dict(numel=(i64 * 2)(-1, 16)), dict(codes=b"\0\2"), dict(n=0), dict(n=-1), dict(kind=3), dict(kind=-1),
                dict(limit=-1.0), dict(limit=math.nan), dict(clip=3), dict(clip=-1), dict(out=None), dict(ws=None),
-               dict(wsb=wsb - 1), dict(ptrs=None), dict(ptrs=(u64 * 2)(1 << 63, 8192))):
+               dict(wsb=wsb - 1), dict(ptrs=None), dict(ptrs=(u64 * 2)(1 << 63, 1 << 20))):
         assert norm(**kw) == 1, kw
-    assert norm(ptrs=(u64 * 2)(4098, 8192)) == 2             # fp32 at a 2-byte address
-    assert norm(ptrs=(u64 * 2)(4097, 8192), codes=b"\1\0") == 2
+    assert norm(ptrs=(u64 * 2)(4098, 1 << 20)) == 2          # fp32 at a 2-byte address
+    assert norm(ptrs=(u64 * 2)(4097, 1 << 20), codes=b"\1\0") == 2
 
 
 def test_clip_refusals():

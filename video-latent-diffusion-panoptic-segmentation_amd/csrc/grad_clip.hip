@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256) void scale_joined(const S t, const double* __r
 
 // Few gradients in one launch of one block: every thread holds up to UNITS packs between the norm and the product,
 // so nothing is read twice.  A unit is a wave's 64 packs of one span; `span` names each unit's.
-constexpr int UNITS = 5, SMALL_WAVES = 16, SMALL_SPANS = 208;
+constexpr int UNITS = 5, SMALL_WAVES = 16, SMALL_SPANS = 64;
 struct SmallTable {
   Entry e[SMALL_SPANS];                    // chunk0: the span's first unit
   uint8_t span[UNITS * SMALL_WAVES];
@@ -347,13 +347,15 @@ int launch_small(const SmallTable& t, int norm_type, float max_norm, int clip, f
 // fp32 ones of the size that the call may take
 extern "C" size_t ldm_grad_norm_workspace_bytes(const int64_t* numel, int ntensors) {
   if (!numel || ntensors <= 0) return 0;
-  int64_t total = 0, small = 0, large = 0;
+  int64_t total = 0, small = 0, large = 0, units = 0;
   for (int i = 0; i < ntensors; ++i)
     if (numel[i] > 0) {
       total += numel[i];
+      units += (numel[i] * 4 + 1023) / 1024;
       small += (numel[i] + chunk_of<float, SMALL_PACKS>() - 1) / chunk_of<float, SMALL_PACKS>();
       large += (numel[i] + chunk_of<float, LARGE_PACKS>() - 1) / chunk_of<float, LARGE_PACKS>();
     }
+  if (units <= UNITS * SMALL_WAVES && ntensors <= SMALL_SPANS) return 0;      // one block, whatever the types
   const int64_t chunks = total * 2 < SMALL_BYTES ? small : large;       // 2 bytes an element at least
   return MAX_BLOCKS * sizeof(double) + (entries_of(numel, ntensors) > TABLE ? (size_t)chunks * sizeof(Chunk) : 0);
 }
@@ -400,7 +402,8 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
                              int64_t workspace_bytes, ldm_stream_t stream) {
   if (!ptrs || !numel || !dtypes || !out || ntensors <= 0 || clip < 0 || clip > 2) return LDM_ERR_ARG;
   if (norm_type < LDM_NORM_2 || norm_type > LDM_NORM_1 || !(max_norm >= 0.0)) return LDM_ERR_ARG;
-  if (!workspace || workspace_bytes < (int64_t)ldm_grad_norm_workspace_bytes(numel, ntensors)) return LDM_ERR_ARG;
+  const int64_t need = (int64_t)ldm_grad_norm_workspace_bytes(numel, ntensors);
+  if (need && (!workspace || workspace_bytes < need)) return LDM_ERR_ARG;
   // Tensors in the order of their addresses; those that lie back to back (views of a bucket) are one span.
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(workspace);

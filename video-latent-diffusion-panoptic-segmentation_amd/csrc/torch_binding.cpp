@@ -324,7 +324,8 @@ PyObject* label_positions(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 // ------------------------------------------------------------------------------------ gradient norms
 // (tensors, of_params, norm_type code, max_norm, clip, out | None): the norm and the factor of `tensors` (or, with
-// of_params, of the gradients that they have), clip as in ldm_grad_norm -> (norm, out), or None without a gradient
+// of_params, of the gradients that they have), clip as in ldm_grad_norm -> the norm, or (norm, out) where clip is 0
+// and out None; None without a gradient
 PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   TORCH_CHECK(nargs == 6 && p_norm, "grad_norm: 6 arguments after init()");
@@ -381,6 +382,7 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   TORCH_CHECK_VALUE(rc != LDM_ERR_OVERLAP,
                     "gradients overlap in memory (the same gradient twice, or views of one another)");
   check_status(rc, "ldm_grad_norm");
+  if (clip || args[5] != Py_None) return THPVariable_Wrap(out.select(0, 0));
   return Py_BuildValue("NN", THPVariable_Wrap(out.select(0, 0)), THPVariable_Wrap(out));
   END_HANDLE_TH_ERRORS
 }

@@ -1928,8 +1928,8 @@ NORM_TYPES = {2.0: 0, math.inf: 1, 1.0: 2}
 
 
 def _grad_norm(tensors, of_params, norm_type, max_norm, clip, out=None):
-    """(norm, [norm, factor]) of tensors, or of their gradients; None where there are none.  ``clip`` as in
-    ldm_grad_norm."""
+    """Norm of tensors, or of their gradients; None where there are none.  ``clip`` as in ldm_grad_norm; with 0
+    (norm, [norm, factor]), whose second ``out`` of a later call with 2 takes."""
     if isinstance(tensors, torch.Tensor):
         tensors = (tensors,)
     kind = NORM_TYPES.get(norm_type)
@@ -1949,4 +1949,4 @@ def clip_grads(grads, max_norm, norm_type=2.0):
     """grad_norm, then every gradient times min(1, max_norm / (norm + 1e-6)) in place (nothing is written
     where the factor is 1) -> the norm before clipping.  Gradients must not overlap."""
     r = _grad_norm(grads, False, norm_type, max_norm, 1)
-    return torch.tensor(0.0) if r is None else r[0]
+    return torch.tensor(0.0) if r is None else r

@@ -18,7 +18,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     norm_type = float(norm_type)
     if not error_if_nonfinite:
         r = K._grad_norm(parameters, True, norm_type, max_norm, 1)
-        return torch.tensor(0.0) if r is None else r[0]
+        return torch.tensor(0.0) if r is None else r
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     r = K._grad_norm(parameters, True, norm_type, max_norm, 0)
     if r is None:
