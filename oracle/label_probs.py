@@ -73,4 +73,5 @@ def label_log_probs_bwd(logits, labels, d_log_prob, d_entropy, *, dim=1, tempera
     if d_entropy is not None:
         h = f["entropy"].unsqueeze(-1)
         d -= d_entropy.double().cpu().unsqueeze(-1) * torch.where(p == 0, torch.zeros_like(p), p * (log_p + h))
-    return (d / temperature).movedim(-1, dim)
+    left = _left(logits, dim, class_mask)[1]
+    return torch.where(left, d / temperature, torch.zeros_like(d)).movedim(-1, dim)

@@ -15,7 +15,8 @@ U = 2.0 ** -24
 
 def chain(logits, dim):
     """Terms that are summed in sequence, at most: every class where they are strided (a thread has a position); of
-    adjacent classes 1/256 of them, a row being a block's, and no more than 512 where it is shorter."""
+    adjacent classes 1/256 of them, a row being a block's, and no more than 512 where it is shorter (a wave's 64 lanes
+    share up to 8192)."""
     C = logits.shape[dim]
     return C if logits.stride(dim) != 1 or C < 512 else max(512, C // 256 + 64)
 

@@ -79,6 +79,28 @@ def test_rows(N, C, topk, T, dtype):
     _run(x.to(DEV), y.to(DEV), topk=topk, temperature=T)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape,topk", [
+    ((2049, 1025), 16), ((2100, 1031), 0), ((2051, 2001), 3), ((2048, 4103), 8),       # a wave to a row
+    ((2, 30, 257, 257), 8), ((1, 17, 363, 365), 16), ((3, 16, 211, 211), 4),           # a thread to a position
+])
+def test_many_positions(shape, topk, dtype):
+    """Calls that fill the card with one wave to a row, or one thread to a position: with a mask for each row (none,
+    one class, half of them left), NaN and infinities where it leaves classes out and in a few rows where it does not."""
+    g = torch.Generator().manual_seed(sum(shape))
+    N, C = shape[:2]
+    x = (torch.randn(shape, generator=g) * 3).to(DT[dtype])
+    x[:, C // 3][torch.rand(shape[:1] + shape[2:], generator=g) < 0.01] = math.nan
+    x[:, C // 2][torch.rand(shape[:1] + shape[2:], generator=g) < 0.01] = math.inf
+    x[:, C - 1][torch.rand(shape[:1] + shape[2:], generator=g) < 0.01] = -math.inf
+    y = _labels(shape[:1] + shape[2:], C, g)
+    _run(x.to(DEV), y.to(DEV), topk=topk)
+    m = _mask(N, C, g)
+    x = torch.where(m.view(N, C, *[1] * (len(shape) - 2)), x, torch.full((), math.nan, dtype=x.dtype))
+    out, d = _run(x.to(DEV), y.to(DEV), topk=topk, class_mask=m.to(DEV), temperature=0.5)
+    assert (out.entropy[0] == 0).all() and (d[0] == 0).all()
+
+
 def _views(dtype):
     g = torch.Generator().manual_seed(11)
     mk = lambda *s: (torch.randn(*s, generator=g) * 3).to(dtype).to(DEV)  # noqa: E731
