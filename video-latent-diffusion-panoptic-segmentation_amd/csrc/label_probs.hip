@@ -340,8 +340,8 @@ __global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
 
 // Long rows of adjacent classes: a block has one segment of one row, its threads packs of VEC classes, UNR of them
 // in flight.  One segment to a row: the block finishes it.  More: what the segments come to goes to the workspace
-// and probs_join finishes the row.  4096 x 16384 fp32: 57 us (4.7 TB/s), bf16 31 us (4.3 TB/s, the vector pipe); four
-// packs in flight: 55 and 31, but rows of 4096 took 68 us for 44.  One row of 65537 fp32: 6 us in 65 segments, with 8
+// and probs_join finishes the row.  4096 x 16384 fp32: 57 us (4.7 TB/s), bf16 31 us back to back (4.3 TB/s, the vector pipe), 38
+// one at a time; four packs in flight: 55 and 31, but rows of 4096 took 68 us for 44.  One row of 65537 fp32: 6 us in 65 segments, with 8
 // alternatives 12 us, half of it in each launch.
 struct Part { float m, r, t; int nan; };
 // (key, class) as one number: larger is earlier in the answer (larger key, then lower class), 0 is none
@@ -658,21 +658,33 @@ __device__ __forceinline__ int list_classes(const uint8_t* mask, int classes, ui
 // own, so that a block's classes are one list (or one run of all)
 struct Tiling { int64_t run; unsigned blocks; };
 
+// Block b of a launch runs on XCD b mod 8, each with an L2 of its own.  The tile it takes instead of the b-th: `near`
+// neighbours in a row go to one XCD, so that a line which two of them share, their planes being at any address, is
+// fetched once.  1 x 128 x 187 x 613 fp32 split: 17 us with an eighth of the launch in a row, 20 us in launch order;
+// not split, 16 in a row: 1 x 64 x 375 x 1242 fp32 29.7 us for 31.2, 1 x 19 x 512 x 1024 15.9 for 17.7, and 1 % more
+// for 8 x 128 x 256 x 256, which has no shared lines (10 % more with an eighth of the launch in a row).
+__device__ __forceinline__ unsigned tile_of(unsigned b, unsigned all, unsigned near) {
+  const unsigned group = 8 * near, first = b / group * group, r = b - first;
+  return first + group > all ? b : first + (r & 7) * near + (r >> 3);
+}
+
 // Forward over strided classes: a thread has one position and UNR classes of it in registers at a time (their loads
 // are in flight together and the maximum's move costs one rescale); a wave reads 64 neighbours of each class plane.
 // With SPLIT the block's four waves have the same 64 positions and a quarter of the classes each, joined through
 // LDS: few positions still fill the card.  LISTED: only the planes of classes that the mask leaves in are read.
 // 8 x 128 x 256 x 256 fp32 frames with 4 alternatives: 55 us (5.2 TB/s); four positions a thread took 70 us, fewer
 // waves of which each waits for 256 positions' lists.  Of unrelated neighbours the lists cost 81 us, none 58.
-// 16 x 128 x 128 x 128 bf16 with 70 % of the classes left: 18 us listed, 35 us with every plane read and tested.
+// 16 x 128 x 128 x 128 bf16 with 70 % of the classes left: 19 us listed, 35 us with every plane read and tested; 16
+// classes in registers take 2 to 6 % less of the wide calls and 20 % more of the narrow ones.
 // 1 x 400 x 40 x 50 fp32: 9.6 us split, 19.1 us not.
 template <typename T, int K, bool SPLIT, bool LISTED>
 __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling tile) {
   constexpr int UNR = 8;
   __shared__ uint16_t list[LISTED ? LIST : 1];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const unsigned row = LISTED ? blockIdx.x / tile.blocks : 0;
-  const int64_t block = LISTED ? blockIdx.x - row * tile.blocks : blockIdx.x;
+  const unsigned id = tile_of(blockIdx.x, gridDim.x, SPLIT ? max(1u, gridDim.x / 8) : 16);
+  const unsigned row = LISTED ? id / tile.blocks : 0;
+  const int64_t block = LISTED ? id - row * tile.blocks : id;
   const int64_t want = SPLIT ? block * 64 + lane : block * 256 + threadIdx.x;
   const bool live = want < tile.run && row * tile.run + want < a.positions;
   int n = a.classes;
@@ -814,12 +826,15 @@ __device__ __forceinline__ float grad_of(const BwdArgs<T>& a, const RowGrad& g, 
 // neighbours of each class plane.  UNIFORM: a block's positions share a row of the class mask, whose bits for the
 // span every wave gathers once; planes that it leaves out are not read.  8 x 128 x 256 x 256: fp32 100 us (5.4 TB/s),
 // bf16 63 us (4.3 TB/s); spans of 8, 113 and 84 us: a position's 16 bytes of sums are read once a span.  Four
-// positions a thread: 119 and 74 us.
+// positions a thread: 119 and 74 us.  Planes that do not begin on a line of 128 bytes are walked by tile_of (1 x 64 x
+// 375 x 1242: fp32 55 us for 60, bf16 34 for 37; the aligned calls above would take 2 % more).
 template <typename T, bool UNIFORM>
 __global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, const Tiling tile, int span) {
   constexpr int UNR = 8;
-  const unsigned row = UNIFORM ? blockIdx.x / tile.blocks : 0;
-  const int64_t want = (int64_t)(UNIFORM ? blockIdx.x - row * tile.blocks : blockIdx.x) * 256 + threadIdx.x;
+  const bool apart = ((uint64_t)a.x | (uint64_t)a.sc * sizeof(T)) % 128 == 0;
+  const unsigned id = apart ? blockIdx.x : tile_of(blockIdx.x, gridDim.x, 16);
+  const unsigned row = UNIFORM ? id / tile.blocks : 0;
+  const int64_t want = (int64_t)(UNIFORM ? id - row * tile.blocks : id) * 256 + threadIdx.x;
   const int c0 = blockIdx.y * span, c1 = min(a.classes, c0 + span);
   uint64_t bits = ~0ull;
   if (UNIFORM) {
