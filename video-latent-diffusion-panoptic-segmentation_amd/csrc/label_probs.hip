@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -674,8 +675,9 @@ __device__ __forceinline__ unsigned tile_of(unsigned b, unsigned all, unsigned n
 // LDS: few positions still fill the card.  LISTED: only the planes of classes that the mask leaves in are read.
 // 8 x 128 x 256 x 256 fp32 frames with 4 alternatives: 55 us (5.2 TB/s); four positions a thread took 70 us, fewer
 // waves of which each waits for 256 positions' lists.  Of unrelated neighbours the lists cost 81 us, none 58.
-// 16 x 128 x 128 x 128 bf16 with 70 % of the classes left: 19 us listed, 35 us with every plane read and tested; 16
-// classes in registers take 2 to 6 % less of the wide calls and 20 % more of the narrow ones.
+// 16 x 128 x 128 x 128 bf16 with 70 % of the classes left: 19 us listed, 35 us with every plane read and tested.
+// Unsplit bf16 takes 16 classes at a time: as many bytes in flight as 8 of fp32, and half the rescales (8 x 128 x 256 x
+// 256: 36.4 us for 39.4); fp32 gains nothing by it and split calls lose 3 %.
 // 1 x 400 x 40 x 50 fp32: 9.6 us split, 19.1 us not.
 template <typename T, int K, bool SPLIT, bool LISTED>
 __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling tile) {
@@ -706,30 +708,37 @@ __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling t
   TopValues<K> top;
   top.clear();
   bool nan = false;
-  auto chunk = [&](const int (&cls)[UNR], float (&f)[UNR]) {
+  auto chunk = [&](auto& cls, auto& f) {
+    constexpr int N = sizeof(f) / sizeof(float);
 #pragma unroll
-    for (int u = 0; u < UNR; ++u) {
+    for (int u = 0; u < N; ++u) {
       if constexpr (K > 0)
         if (__any(f[u] > top.v[K - 1])) top.add(f[u], cls[u]);
       nan |= f[u] != f[u];
     }
-    s.template add_all<UNR>(f, a.c2);
+    s.template add_all<N>(f, a.c2);
   };
   auto class_at = [&](int i) { return LISTED ? __builtin_amdgcn_readfirstlane((int)list[i]) : i; };
   int c = c0;
-  if (LISTED || !mask)
-    for (; c + UNR <= c1; c += UNR) {
-      T v[UNR];
-      float f[UNR];
-      int cls[UNR];
+  auto whole = [&](auto width) {
+    constexpr int N = decltype(width)::value;
+    for (; c + N <= c1; c += N) {
+      T v[N];
+      float f[N];
+      int cls[N];
 #pragma unroll
-      for (int u = 0; u < UNR; ++u) cls[u] = class_at(c + u);
+      for (int u = 0; u < N; ++u) cls[u] = class_at(c + u);
 #pragma unroll
-      for (int u = 0; u < UNR; ++u) v[u] = x[cls[u] * a.sc];
+      for (int u = 0; u < N; ++u) v[u] = x[cls[u] * a.sc];
 #pragma unroll
-      for (int u = 0; u < UNR; ++u) f[u] = to_f(v[u]);
+      for (int u = 0; u < N; ++u) f[u] = to_f(v[u]);
       chunk(cls, f);
     }
+  };
+  if (LISTED || !mask) {
+    if constexpr (sizeof(T) == 2 && !SPLIT) whole(std::integral_constant<int, 16>());
+    whole(std::integral_constant<int, UNR>());
+  }
   for (; c < c1; c += UNR) {
     T v[UNR];
     float f[UNR];
