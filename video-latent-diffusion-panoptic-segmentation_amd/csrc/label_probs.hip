@@ -831,19 +831,20 @@ __device__ __forceinline__ float grad_of(const BwdArgs<T>& a, const RowGrad& g, 
   return (c == g.label ? g.gl : 0.f) - p * w;
 }
 
-// Backward over strided classes: a thread has one position and `span` <= 64 classes, a wave reads and writes 64
-// neighbours of each class plane.  UNIFORM: a block's positions share a row of the class mask, whose bits for the
+// Backward over strided classes: a thread has PV positions (bf16 two side by side, fp32 one) and `span` <= 64 classes, a
+// wave reads and writes 64 PV neighbours of each class plane.  UNIFORM: a block's positions share a row of the class mask, whose bits for the
 // span every wave gathers once; planes that it leaves out are not read.  8 x 128 x 256 x 256: fp32 100 us (5.4 TB/s),
-// bf16 63 us (4.3 TB/s); spans of 8, 113 and 84 us: a position's 16 bytes of sums are read once a span.  Four
-// positions a thread: 119 and 74 us.  Planes that do not begin on a line of 128 bytes are walked by tile_of (1 x 64 x
+// bf16 60 us (4.5 TB/s); spans of 8, 113 and 84 us: a position's 16 bytes of sums are read once a span.  Four
+// positions a thread: 119 and 74 us; bf16 with one: 64 us, and 16 x 128 x 128 x 128 with 70 % of the classes 37 us for
+// 30, but 16 x 4 x 512 x 512 38 us for 42.  Planes that do not begin on a line of 128 bytes are walked by tile_of (1 x 64 x
 // 375 x 1242: fp32 55 us for 60, bf16 34 for 37; the aligned calls above would take 2 % more).
-template <typename T, bool UNIFORM>
+template <typename T, bool UNIFORM, int PV>
 __global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, const Tiling tile, int span) {
   constexpr int UNR = 8;
   const bool apart = ((uint64_t)a.x | (uint64_t)a.sc * sizeof(T)) % 128 == 0;
   const unsigned id = apart ? blockIdx.x : tile_of(blockIdx.x, gridDim.x, 16);
   const unsigned row = UNIFORM ? id / tile.blocks : 0;
-  const int64_t want = (int64_t)(UNIFORM ? id - row * tile.blocks : id) * 256 + threadIdx.x;
+  const int64_t want = ((int64_t)(UNIFORM ? id - row * tile.blocks : id) * 256 + threadIdx.x) * PV;
   const int c0 = blockIdx.y * span, c1 = min(a.classes, c0 + span);
   uint64_t bits = ~0ull;
   if (UNIFORM) {
@@ -856,16 +857,18 @@ __global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, cons
   const T* x = a.x + place.at(a.s0, a.s1, a.s2);
   T* dx = a.dx + place.at(a.o0, a.o1, a.o2);
   const uint8_t* mask = !UNIFORM && a.mask ? a.mask + quotient(pos, a.mask_div, a.positions) * a.mask_stride : nullptr;
-  T v[UNR];
+  Pack<T, PV> v[UNR];
   auto load = [&](int c) {
 #pragma unroll
     for (int u = 0; u < UNR; ++u) {
       const int cu = min(c + u, c1 - 1);
-      if (!UNIFORM || bits >> (cu - c0) & 1) v[u] = x[cu * a.sc];
+      if (!UNIFORM || bits >> (cu - c0) & 1) v[u] = load_pack<T, PV>(x + cu * a.sc);
     }
   };
   load(c0);                        // under way before what the position's sums need
-  const RowGrad g = row_grad(a, pos);
+  RowGrad g[PV];
+#pragma unroll
+  for (int i = 0; i < PV; ++i) g[i] = row_grad(a, pos + i);
   for (int c = c0; c < c1; c += UNR) {
     if (c > c0) load(c);
 #pragma unroll
@@ -873,7 +876,10 @@ __global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, cons
       const int cu = c + u;
       if (cu >= c1) break;
       const bool in = UNIFORM ? bits >> (cu - c0) & 1 : !mask || mask[cu];
-      dx[cu * a.oc] = from_f<T>(in ? grad_of(a, g, to_f(v[u]), cu) : 0.f);
+      Pack<T, PV> d;
+#pragma unroll
+      for (int i = 0; i < PV; ++i) d.v[i] = from_f<T>(in ? grad_of(a, g[i], to_f(v[u].v[i]), cu) : 0.f);
+      store_pack<T, PV>(dx + cu * a.oc, d);
     }
   }
 }
@@ -1036,6 +1042,26 @@ int launch(const Args& a, void* ws, hipStream_t s) {
   return LDM_OK;
 }
 
+template <typename T, int PV>
+int launch_bwd_planes(const BwdArgs<T>& a, int64_t n, hipStream_t s) {
+  // 32 classes to a thread, or down to 8 where the card would have less than 12 waves a CU
+  int span = 32;
+  while (span > 8 && n / 64 / PV * ((a.classes + span - 1) / span) < 12 * 256) span /= 2;
+  const unsigned spans = (unsigned)((a.classes + span - 1) / span);
+  if (spans > 65535 || (n + 255) / 256 > MOST_BLOCKS) return LDM_ERR_ARG;
+  Tiling t;
+  int64_t rows;
+  if (mask_runs(a.mask, a.mask_div, n, 256 * PV, &t, &rows)) {
+    hipLaunchKernelGGL((probs_bwd_planes<T, true, PV>), dim3((unsigned)(rows * t.blocks), spans), dim3(256), 0, s, a, t, span);
+  } else {
+    t.run = n;
+    t.blocks = (unsigned)((n + 256 * PV - 1) / (256 * PV));
+    hipLaunchKernelGGL((probs_bwd_planes<T, false, PV>), dim3(t.blocks, spans), dim3(256), 0, s, a, t, span);
+  }
+  LDM_CHECK_LAUNCH();
+  return LDM_OK;
+}
+
 template <typename T>
 int launch_bwd(const ldm_label_probs_bwd_params* p, int64_t n, hipStream_t s) {
   BwdArgs<T> a;
@@ -1067,22 +1093,12 @@ int launch_bwd(const ldm_label_probs_bwd_params* p, int64_t n, hipStream_t s) {
     LDM_CHECK_LAUNCH();
     return LDM_OK;
   }
-  // 32 classes to a thread, or down to 8 where the card would have less than 12 waves a CU
-  int span = 32;
-  while (span > 8 && n / 64 * ((a.classes + span - 1) / span) < 12 * 256) span /= 2;
-  const unsigned spans = (unsigned)((a.classes + span - 1) / span);
-  if (spans > 65535 || (n + 255) / 256 > MOST_BLOCKS) return LDM_ERR_ARG;
-  Tiling t;
-  int64_t rows;
-  if (mask_runs(a.mask, a.mask_div, n, 256, &t, &rows)) {
-    hipLaunchKernelGGL((probs_bwd_planes<T, true>), dim3((unsigned)(rows * t.blocks), spans), dim3(256), 0, s, a, t, span);
-  } else {
-    t.run = n;
-    t.blocks = (unsigned)((n + 255) / 256);
-    hipLaunchKernelGGL((probs_bwd_planes<T, false>), dim3(t.blocks, spans), dim3(256), 0, s, a, t, span);
+  if constexpr (sizeof(T) == 2) {
+    // pairs of positions side by side, in one row of the mask; of few classes they would only halve the waves
+    const bool whole = a.n2 % 2 == 0 && (!a.mask || a.mask_div >= n || a.mask_div % 2 == 0);
+    if (a.s2 == 1 && a.o2 == 1 && whole && a.classes >= 16) return launch_bwd_planes<T, 2>(a, n, s);
   }
-  LDM_CHECK_LAUNCH();
-  return LDM_OK;
+  return launch_bwd_planes<T, 1>(a, n, s);
 }
 
 bool bad_temperature(float t) { return !(t >= 1e-4f && t <= 1e4f); }
