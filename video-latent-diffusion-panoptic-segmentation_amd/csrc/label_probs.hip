@@ -675,9 +675,10 @@ __device__ __forceinline__ unsigned tile_of(unsigned b, unsigned all, unsigned n
 // LDS: few positions still fill the card.  LISTED: only the planes of classes that the mask leaves in are read.
 // 8 x 128 x 256 x 256 fp32 frames with 4 alternatives: 55 us (5.2 TB/s); four positions a thread took 70 us, fewer
 // waves of which each waits for 256 positions' lists.  Of unrelated neighbours the lists cost 81 us, none 58.
-// 16 x 128 x 128 x 128 bf16 with 70 % of the classes left: 19 us listed, 35 us with every plane read and tested.
+// 16 x 128 x 128 x 128 bf16 with 70 % of the classes left: 17.5 us listed, 35 us with every plane read and tested.
 // Unsplit bf16 takes 16 classes at a time: as many bytes in flight as 8 of fp32, and half the rescales (8 x 128 x 256 x
-// 256: 36.4 us for 39.4); fp32 gains nothing by it and split calls lose 3 %.
+// 256: 36.4 us for 39.4); fp32 gains nothing by it and split calls lose 3 %.  Two positions a
+// thread: 42 us.
 // 1 x 400 x 40 x 50 fp32: 9.6 us split, 19.1 us not.
 template <typename T, int K, bool SPLIT, bool LISTED>
 __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling tile) {
