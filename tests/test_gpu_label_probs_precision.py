@@ -1,0 +1,104 @@
+"""Label probabilities at bounds that do not grow with the number of classes and that are relative to what they bound
+(derived in label_probs_bounds.py)."""
+import math
+
+import pytest
+import torch
+
+from label_probs_bounds import Row, within
+from ldmseg.ops import native as K
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _row(kind, C, gen):
+    if kind == "equal":
+        return torch.zeros(C)
+    if kind == "gap":                       # one class against all others, together as likely as it
+        x = torch.full((C,), -math.log(C))
+        x[C // 3] = 0.0
+        return x
+    if kind == "far_gap":
+        x = torch.full((C,), -15.0)
+        x[-1] = 0.0
+        return x
+    if kind == "rising":
+        return torch.arange(C) * 1e-6
+    if kind == "rising_fast":
+        return torch.arange(C) * 1e-4
+    if kind == "falling":
+        return torch.arange(C) * -1e-5
+    return torch.randn(C, generator=gen) * 2
+
+
+KINDS = ["equal", "gap", "far_gap", "rising", "rising_fast", "falling", "normal"]
+
+
+def _check_forward(x, y, dim, topk, mask=None, temperature=1.0):
+    out = K.label_log_probs(x, y, dim=dim, topk=topk, class_mask=mask, temperature=temperature, want_stats=True)
+    row = Row(x, dim, temperature, mask)
+    within(out.entropy, row.H, row.err_H(), "entropy")
+    ids = y.unsqueeze(-1)
+    within(out.log_prob.unsqueeze(-1), row.log_p(ids), row.err_log_p(ids), "log_prob")
+    if topk:
+        ids = out.top_ids.movedim(dim, -1).long()
+        within(out.top_log_probs.movedim(dim, -1), row.log_p(ids), row.err_log_p(ids), "top_log_probs")
+    return out, row
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("C", [700, 4096, 16384, 50001, 131072])
+def test_sums_over_many_strided_classes(C, dtype):
+    """Equal gaps round in one direction all the way, and a rising row moves its maximum at every class: neither may
+    show in the sums as their number grows."""
+    g = torch.Generator().manual_seed(C)
+    N = 70 if C <= 4096 else 10                                 # enough of them for a list of the classes left
+    x = torch.stack([_row(k, C, g) for k in KINDS]).to(DT[dtype]).unsqueeze(2).expand(-1, -1, N).contiguous().to(DEV)
+    y = torch.randint(0, C, (len(KINDS), N), generator=g).to(DEV)
+    _check_forward(x, y, 1, 3)
+    mask = torch.rand(len(KINDS), C, generator=g) < 0.8
+    mask[:, C // 3] = True
+    mask.scatter_(1, y.cpu(), True)
+    _check_forward(x, y, 1, 0, mask.to(DEV))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_sums_with_a_thread_to_a_position(masked, dtype):
+    """131200 positions of 2048 classes: one thread has all classes of a position.  Every position has the same row."""
+    C, N = 2048, 131200
+    g = torch.Generator().manual_seed(1)
+    for kind in ("equal", "gap", "rising"):
+        one = _row(kind, C, g).to(DT[dtype]).to(DEV)
+        mask = None
+        if masked:
+            mask = torch.ones(1, C, dtype=torch.bool, device=DEV)
+            mask[:, 5::3] = False
+            mask[:, C // 3] = True
+        out = K.label_log_probs(one.view(1, C, 1).expand(1, C, N).contiguous(),
+                                torch.full((1, N), C // 3, device=DEV), class_mask=mask)
+        row = Row(one.view(1, C, 1), 1, class_mask=mask)
+        ids = torch.full((1, 1, 1), C // 3, device=DEV)
+        for at in (0, 1, N // 2, N - 1):
+            within(out.entropy[:, at:at + 1], row.H, row.err_H(), "entropy")
+            within(out.log_prob[:, at:at + 1, None], row.log_p(ids), row.err_log_p(ids), "log_prob")
+        assert (out.entropy == out.entropy[0, 0]).all() and (out.log_prob == out.log_prob[0, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("C,N", [(1001, 7), (8192, 2051), (20000, 600), (1_000_003, 7)])
+def test_sums_over_many_adjacent_classes(C, N, dtype):
+    g = torch.Generator().manual_seed(C)
+    x = torch.stack([_row(k, C, g) for k in KINDS]).to(DT[dtype]).to(DEV)
+    x = x.repeat(-(-N // len(KINDS)), 1)[:N]
+    y = torch.randint(0, C, (N,), generator=g).to(DEV)
+    if N * C > 1 << 24:                                         # only some of the rows' references fit
+        out = K.label_log_probs(x, y)
+        keep = torch.cat([torch.arange(7), torch.arange(N - 7, N)]).to(DEV)
+        row, ids = Row(x[keep]), y[keep, None]
+        within(out.entropy[keep], row.H, row.err_H(), "entropy")
+        within(out.log_prob[keep, None], row.log_p(ids), row.err_log_p(ids), "log_prob")
+    else:
+        _check_forward(x, y, 1, 3)

@@ -35,7 +35,7 @@ struct Args {
   int has_ignore;
   const uint8_t* mask;
   int64_t mask_stride, mask_div, inner;
-  float c2, inv_t;                 // log2(e) / T, 1 / T
+  float c2, inv_t, slack;          // log2(e) / T, 1 / T, T ln 2
   float *lp, *ent, *top_lp, *stats;
   int32_t* top_id;
   int k;
@@ -71,42 +71,14 @@ __device__ __forceinline__ float raw_min(float a, float b) {
   return r;
 }
 
-// running maximum and sums of one set of logits; the maximum's own term is in neither sum
+// maximum and sums of one set of logits; the maximum's own term is in neither sum
 struct Soft {
   float m, r, t;
   __device__ __forceinline__ void clear() { m = -INFINITY; r = t = 0.f; }
-  __device__ __forceinline__ void rescale(float to, float c2) {   // sums relative to `to` >= m, to > -inf
+  __device__ __forceinline__ void rescale(float to, float c2) {   // sums relative to `to` > -inf
     const float d = fmaxf(m - to, LOWEST), s = exp2_fast(d * c2);
     t = s * t + (s * d) * r;
     r *= s;
-  }
-  __device__ __forceinline__ void add(float x, float c2) {        // x is no NaN
-    const float hi = fmaxf(m, x), lo = fminf(m, x), to = hi == -INFINITY ? 0.f : hi;
-    rescale(to, c2);
-    const float d = fmaxf(lo - to, LOWEST), e = exp2_fast(d * c2);
-    r += e;
-    t = fmaf(d, e, t);
-    m = hi;
-  }
-  // N logits at once, no NaN heeded: one move of the maximum.  It is carried through them: what each passes on is
-  // the lesser of the two, so the set {m, f} becomes {new m} and the f that are left to sum.
-  template <int N> __device__ __forceinline__ void add_all(float (&f)[N], float c2) {
-    float hi = m;
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const float v = f[u];
-      f[u] = raw_min(hi, v);
-      hi = raw_max(hi, v);
-    }
-    const float to = hi == -INFINITY ? 0.f : hi;
-    rescale(to, c2);
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const float d = fmaxf(f[u] - to, LOWEST), e = exp2_fast(d * c2);
-      r += e;
-      t = fmaf(d, e, t);
-    }
-    m = hi;
   }
   __device__ __forceinline__ void join(const Soft& o, float c2) { // o's classes and these
     const float hi = fmaxf(m, o.m), lo = fminf(m, o.m), to = hi == -INFINITY ? 0.f : hi;
@@ -117,6 +89,67 @@ struct Soft {
     r += b.r + e;
     t += b.t + d * e;
     m = hi;
+  }
+};
+
+// The same of a thread's logits while it walks them.  Their number does not show in the sums' rounding: a chunk's
+// terms are added up by themselves, FOLD chunks in fp32 and those in fp64 (131072 strided logits of one value but the
+// maximum in one accumulator: 5e-4 off).  R and T are relative to `ref`, a former maximum that is replaced where the
+// maximum has passed it by a factor of two: what came before then loses half its weight, and with it the rounding of
+// its product with e^(ref - m), however often a slowly rising row does this.  Threads of no more than FOLD chunks have
+// FOLDS false: 1 x 19 x 512 x 1024 fp32 12.9 us, 13.7 us with the folds' code and registers beside the loop.
+constexpr int FOLD = 32;
+template <bool FOLDS> struct Run {
+  float m, r, t, ref;
+  double R, T;
+  int chunks;
+  __device__ __forceinline__ void clear() { m = ref = -INFINITY; r = t = 0.f; R = T = 0.0; chunks = 0; }
+  // N logits, no NaN heeded: one move of the maximum.  It is carried through them: what each passes on is the lesser
+  // of the two, so the set {m, f} becomes {new m} and the f that are left to sum.
+  template <int N> __device__ __forceinline__ void add_all(float (&f)[N], float c2, float slack) {
+    float hi = m;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const float v = f[u];
+      f[u] = raw_min(hi, v);
+      hi = raw_max(hi, v);
+    }
+    const float to = hi == -INFINITY ? 0.f : hi, dm = fmaxf(m - to, LOWEST), s = exp2_fast(dm * c2);
+    float rr, tt;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const float d = fmaxf(f[u] - to, LOWEST), e = exp2_fast(d * c2);
+      rr = u ? rr + e : e;
+      tt = u ? fmaf(d, e, tt) : d * e;
+    }
+    t = fmaf(s, t, fmaf(s * dm, r, tt));
+    r = fmaf(s, r, rr);
+    m = hi;
+    if constexpr (FOLDS)
+      if (++chunks % FOLD == 0) fold(c2, slack);
+  }
+  __device__ __forceinline__ void fold(float c2, float slack) {
+    if (m == -INFINITY) return;                   // nothing so far
+    if (ref == -INFINITY || m > ref + slack) {
+      const float d = fmaxf(ref - m, LOWEST);
+      const double s = exp2_fast(d * c2);
+      T = s * (T + d * R);
+      R *= s;
+      ref = m;
+    }
+    const float d = m - ref;
+    const double s = exp2_fast(d * c2);
+    R += s * r;
+    T += s * ((double)t + (double)d * r);
+    r = t = 0.f;
+  }
+  __device__ __forceinline__ Soft sums(float c2, float slack) {
+    if (!FOLDS || chunks < FOLD || m == -INFINITY) return {m, r, t};
+    fold(c2, slack);
+    Soft s = {ref, (float)R, (float)T};
+    s.rescale(m, c2);
+    s.m = m;
+    return s;
   }
 };
 
@@ -500,8 +533,8 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
   RowParts<TOP, WAVES>& mine = sh[WAVES == 1 ? wave : 0];
   Best& best = mine.best[TOP && WAVES == 4 ? wave : 0];
   int count = 0;                   // the wave's candidates
-  Soft s;
-  s.clear();
+  Run<(WAVES > 1)> run;             // a wave's row has 16 chunks at most (WAVE_CLASSES)
+  run.clear();
   uint64_t nans = 0;               // lanes that saw one
   LabelAt l;
   if (segments == 1) l = label_at<T>(a, pos);
@@ -514,7 +547,7 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
     if constexpr (TOP)
       enter_above_bar<N>(best, count, bar, a.k, f, odd >> lane & 1,
                          [&](int i) { return min(at0 + i / VEC * W * VEC, last) + i % VEC; });
-    s.template add_all<N>(f, a.c2);
+    run.template add_all<N>(f, a.c2, a.slack);
   };
   int base = seg * seg_len;        // the same turns in every lane: they exchange values
   if (!mask)
@@ -547,6 +580,7 @@ __global__ __launch_bounds__(256) void probs_rows(const Args a, int segments, in
   }
   uint64_t answer = 0;
   bool nan = nans != 0;
+  Soft s = run.sums(a.c2, a.slack);
   if constexpr (WAVES == 1) {
     s = wave_join(s, a.c2);
     if constexpr (TOP) answer = first_of(lane < count ? best.some[lane] : 0, count, a.k, best.sorted);
@@ -669,6 +703,7 @@ __device__ __forceinline__ unsigned tile_of(unsigned b, unsigned all, unsigned n
   return first + group > all ? b : first + (r & 7) * near + (r >> 3);
 }
 
+constexpr int PLANES_UNR = 8;
 // Forward over strided classes: a thread has one position and UNR classes of it in registers at a time (their loads
 // are in flight together and the maximum's move costs one rescale); a wave reads 64 neighbours of each class plane.
 // With SPLIT the block's four waves have the same 64 positions and a quarter of the classes each, joined through
@@ -680,11 +715,11 @@ __device__ __forceinline__ unsigned tile_of(unsigned b, unsigned all, unsigned n
 // 256: 36.4 us for 39.4); fp32 gains nothing by it and split calls lose 3 %.  Two positions a
 // thread: 42 us.
 // 1 x 400 x 40 x 50 fp32: 9.6 us split, 19.1 us not.
-template <typename T, int K, bool SPLIT, bool LISTED>
+template <typename T, int K, bool SPLIT, bool LISTED, bool FOLDS>
 __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling tile) {
-  constexpr int UNR = 8;
+  constexpr int UNR = PLANES_UNR;
   __shared__ uint16_t list[LISTED ? LIST : 1];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const unsigned id = tile_of(blockIdx.x, gridDim.x, SPLIT ? max(1u, gridDim.x / 8) : 16);
   const unsigned row = LISTED ? id / tile.blocks : 0;
   const int64_t block = LISTED ? id - row * tile.blocks : id;
@@ -704,8 +739,8 @@ __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling t
     y = a.labels[pos];             // its logit is fetched beside the loop, which reads that line as well
     if (y >= 0 && y < a.classes && !(mask && !mask[y])) xy = to_f(x[y * a.sc]);
   }
-  Soft s;
-  s.clear();
+  Run<FOLDS> run;
+  run.clear();
   TopValues<K> top;
   top.clear();
   bool nan = false;
@@ -717,7 +752,7 @@ __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling t
         if (__any(f[u] > top.v[K - 1])) top.add(f[u], cls[u]);
       nan |= f[u] != f[u];
     }
-    s.template add_all<N>(f, a.c2);
+    run.template add_all<N>(f, a.c2, a.slack);
   };
   auto class_at = [&](int i) { return LISTED ? __builtin_amdgcn_readfirstlane((int)list[i]) : i; };
   int c = c0;
@@ -755,6 +790,7 @@ __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling t
     for (int u = 0; u < UNR; ++u) f[u] = in[u] ? to_f(v[u]) : -INFINITY;
     chunk(cls, f);
   }
+  Soft s = run.sums(a.c2, a.slack);
   if constexpr (SPLIT) {
     __shared__ Soft part[4][64];
     __shared__ bool part_nan[4][64];
@@ -951,24 +987,25 @@ bool mask_runs(const void* mask, int64_t mask_div, int64_t positions, int per_bl
   return mask && *rows * t->blocks <= MOST_BLOCKS;
 }
 
-template <typename T, int K, bool SPLIT>
+template <typename T, int K, bool SPLIT, bool FOLDS>
 void launch_planes_as(const Args& a, hipStream_t s) {
   constexpr int PER = SPLIT ? 64 : 256;
   Tiling t;
   int64_t rows;
   if (a.classes <= LIST && mask_runs(a.mask, a.mask_div, a.positions, PER, &t, &rows)) {
-    hipLaunchKernelGGL((probs_planes<T, K, SPLIT, true>), dim3((unsigned)(rows * t.blocks)), dim3(256), 0, s, a, t);
+    hipLaunchKernelGGL((probs_planes<T, K, SPLIT, true, FOLDS>), dim3((unsigned)(rows * t.blocks)), dim3(256), 0, s, a, t);
   } else {
     t.run = a.positions;
     t.blocks = (unsigned)((t.run + PER - 1) / PER);
-    hipLaunchKernelGGL((probs_planes<T, K, SPLIT, false>), dim3(t.blocks), dim3(256), 0, s, a, t);
+    hipLaunchKernelGGL((probs_planes<T, K, SPLIT, false, FOLDS>), dim3(t.blocks), dim3(256), 0, s, a, t);
   }
 }
 template <typename T, int K>
 void launch_planes_split(const Args& a, hipStream_t s) {
   // four waves to 64 positions where whole ones would leave the card with less than 8 waves a CU
-  if (a.positions < 64 * 2048 && a.classes >= 16) launch_planes_as<T, K, true>(a, s);
-  else launch_planes_as<T, K, false>(a, s);
+  if (a.positions < 64 * 2048 && a.classes >= 16) launch_planes_as<T, K, true, true>(a, s);
+  else if (a.classes > FOLD * PLANES_UNR) launch_planes_as<T, K, false, true>(a, s);
+  else launch_planes_as<T, K, false, false>(a, s);
 }
 template <typename T>
 int launch_planes(const Args& a, hipStream_t s) {
@@ -1132,7 +1169,7 @@ extern "C" int ldm_label_log_probs(const ldm_label_probs_params* p, ldm_stream_t
   a.labels = p->labels; a.ignore = p->ignore_label; a.has_ignore = p->has_ignore;
   a.mask = (const uint8_t*)p->class_mask; a.mask_stride = p->mask_stride; a.mask_div = p->mask_div;
   a.inner = p->inner;
-  a.inv_t = 1.f / p->temperature; a.c2 = (float)(1.4426950408889634 / p->temperature);
+  a.inv_t = 1.f / p->temperature; a.c2 = (float)(1.4426950408889634 / p->temperature); a.slack = p->temperature * LN2;
   a.lp = p->log_prob; a.ent = p->entropy; a.top_lp = p->top_log_probs; a.top_id = p->top_ids; a.stats = p->stats;
   a.k = p->topk;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
