@@ -726,7 +726,8 @@ int ldm_adamw(float* param, const float* grad, float* exp_avg, float* exp_avg_sq
  *                top_ids -1 / top_log_probs -inf past the classes with probability.  Entry j of
  *                position p is at (p / inner) * topk * inner + j * inner + p % inner.
  *   stats        NULL, or fp32 [4][positions] for the backward: max logit, log of the sum,
- *                entropy, label (int32 bits; -1: no gradient through log_prob).
+ *                entropy, label (int32 bits; -1: no gradient through log_prob; bit 30: its logit is
+ *                the maximum).
  * A row with no class left (all masked or -inf): entropy 0, ids -1.  NaN or +inf among the
  * classes left: log_prob and entropy NaN.  temperature in [1e-4, 1e4].
  * ldm_label_log_probs_bwd: d_logits = (d_log_prob * (onehot(label) - p) - d_entropy * p * (log p +

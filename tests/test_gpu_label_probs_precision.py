@@ -102,3 +102,41 @@ def test_sums_over_many_adjacent_classes(C, N, dtype):
         within(out.log_prob[keep, None], row.log_p(ids), row.err_log_p(ids), "log_prob")
     else:
         _check_forward(x, y, 1, 3)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("layout", ["planes", "planes_odd", "short_rows", "rows", "long_rows"])
+@pytest.mark.parametrize("T", [1.0, 0.5])
+def test_gradient_of_a_confident_label_keeps_its_digits(layout, T, dtype):
+    """1 - p of the label runs from 0.3 to 1e-12: its gradient is relative to that, also below a rounding of 1, and
+    the row's gradients add up to 0 as far as their type can say."""
+    C = {"planes": 37, "planes_odd": 37, "short_rows": 40, "rows": 700, "long_rows": 3001}[layout]
+    N = 62 if layout != "planes_odd" else 61
+    g = torch.Generator().manual_seed(C)
+    gaps = torch.linspace(2.0, 30.0, N) + math.log(C)
+    x = -gaps.unsqueeze(1) - 2 * torch.rand(N, C, generator=g)
+    y = torch.randint(0, C, (N,), generator=g)
+    x.scatter_(1, y.unsqueeze(1), 0.0)
+    x = (x * T).to(DT[dtype])
+    y[-1] = (y[-1] + 1) % C                                     # one that is not the maximum
+    x[5, (y[5] + 1) % C] = 0.0                                  # two maxima
+    gl = torch.randn(N, generator=g)
+    ge = torch.randn(N, generator=g)
+    ge[::2] = 0
+    if layout.startswith("planes"):
+        xx, yy, dim = x.t().contiguous().unsqueeze(0).to(DEV), y.unsqueeze(0).to(DEV), 1
+        gl, ge = gl.unsqueeze(0), ge.unsqueeze(0)
+    else:
+        xx, yy, dim = x.to(DEV), y.to(DEV), 1
+    gl, ge = gl.to(DEV), ge.to(DEV)
+    out = K.label_log_probs(xx, yy, temperature=T, want_stats=True)
+    for e in (None, ge):
+        d = K.label_log_probs_bwd(xx, out.stats, gl, e, temperature=T)
+        want, tol = Row(xx, dim, T).grad(yy, gl.double(), None if e is None else e.double(), xx.dtype)
+        got = d.movedim(dim, -1)
+        own = torch.zeros_like(want, dtype=torch.bool).scatter_(-1, yy.unsqueeze(-1), True)
+        within(got[own], want[own], tol[own], "the label's gradient")
+        within(got, want, tol, "gradient")
+        if e is None:
+            assert ((got.double().sum(-1)).abs() <= tol.sum(-1)).all()
+            assert (got[own] != 0).all()

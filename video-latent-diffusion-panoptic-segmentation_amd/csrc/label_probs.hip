@@ -182,6 +182,9 @@ __device__ __forceinline__ float log1p_of(float r) {
   return w == 1.f ? r : l * (r * __builtin_amdgcn_rcpf(w - 1.f));
 }
 
+// In the saved label: its logit is the row's maximum.  Classes are numbered below it.
+constexpr int MOST_CLASSES = 1 << 30, LABEL_LEADS = 1 << 30;
+
 // what a position's sums come to
 struct Result { float ls, ent, lp; int label; };
 __device__ __forceinline__ Result result_of(const Args& a, const Soft& s, bool nan, int64_t y, float xy) {
@@ -194,7 +197,8 @@ __device__ __forceinline__ Result result_of(const Args& a, const Soft& s, bool n
   if (!known) q.lp = 0.f;
   else if (!inside || bad) q.lp = none;
   else q.lp = xy == -INFINITY ? -INFINITY : (xy - s.m) * a.inv_t - q.ls;
-  q.label = known && inside && q.lp > -INFINITY ? (int)y : -1;   // NaN > -inf is false: the row is NaN anyway
+  q.label = !(known && inside && q.lp > -INFINITY) ? -1          // NaN > -inf is false: the row is NaN anyway
+            : xy == s.m ? (int)y | LABEL_LEADS : (int)y;
   return q;
 }
 __device__ __forceinline__ void store_top(const Args& a, int64_t pos, int j, int key, int id, const Soft& s, float ls) {
@@ -845,27 +849,44 @@ struct BwdArgs {
   const float *stats, *gl, *ge;
 };
 
-struct RowGrad { float m, ls, ls2, h, gl, ge; int label; };
+// 1 - e^-x, x >= 0, to a few roundings of itself: the exponential's series where the difference would cancel
+// (the first term left out is below 2^-30 of the sum)
+__device__ __forceinline__ float one_minus_exp(float x) {
+  constexpr float C[] = {1.f / 2, 1.f / 6, 1.f / 24, 1.f / 120, 1.f / 720, 1.f / 5040, 1.f / 40320, 1.f / 362880, 1.f / 3628800};
+  float f = C[8];
+#pragma unroll
+  for (int k = 7; k >= 0; --k) f = fmaf(-x, f, C[k]);
+  return x < LN2 ? fmaf(-x * x, f, x) : 1.f - exp2_fast(-x * LOG2E);
+}
+
+// d x_j = (1[j == y] g_y - p_j w_j) / T, w_j = g_l + g_H (log p_j + H) = w0 + w1 z2_j.  Of a label at the row's maximum,
+// 1 - p_y and log p_y + H follow from the row's own sums, 1 - p_y = 1 - e^-ls without a difference of neighbours: g_y is
+// its whole gradient, and its p_y w_y is kept out by an infinite `ls2_y`.  p of any other label is at most 1/2.
+struct RowGrad { float m, ls2, ls2_y, w0, w1, g_y; int label; };
 template <typename T>
 __device__ __forceinline__ RowGrad row_grad(const BwdArgs<T>& a, int64_t pos) {
   RowGrad g;
   g.m = a.stats[pos];
-  g.ls = a.stats[a.positions + pos];
-  g.h = a.stats[2 * a.positions + pos];
-  g.label = __float_as_int(a.stats[3 * a.positions + pos]);
-  g.gl = a.gl && g.label >= 0 ? a.gl[pos] * a.inv_t : 0.f;
-  g.ge = a.ge ? a.ge[pos] * a.inv_t : 0.f;
-  g.ls2 = g.ls * LOG2E;
-  if (g.m == -INFINITY) { g.m = 0.f; g.gl = g.ge = 0.f; }
+  const float ls = a.stats[a.positions + pos], off = a.stats[2 * a.positions + pos] - ls;    // H - ls
+  const int label = __float_as_int(a.stats[3 * a.positions + pos]);
+  const bool leads = label >= 0 && (label & LABEL_LEADS);
+  float gl = a.gl && label >= 0 ? a.gl[pos] * a.inv_t : 0.f, ge = a.ge ? a.ge[pos] * a.inv_t : 0.f;
+  if (g.m == -INFINITY) g.m = gl = ge = 0.f;
+  g.label = label < 0 ? -1 : label & ~LABEL_LEADS;
+  g.ls2 = ls * LOG2E;
+  g.ls2_y = leads ? INFINITY : g.ls2;
+  g.w0 = fmaf(ge, off, gl);
+  g.w1 = ge * LN2;
+  g.g_y = leads ? gl * one_minus_exp(ls) - ge * exp2_fast(-g.ls2) * off : gl;
   return g;
 }
 template <typename T>
 __device__ __forceinline__ float grad_of(const BwdArgs<T>& a, const RowGrad& g, float x, int c) {
   // below 2^-1000 p is 0 and its log stays finite; a row with a NaN or +inf has ls = NaN, and so has every p of it
   const float z2 = fmaxf((x - g.m) * a.c2, -1000.f);
-  const float p = exp2_fast(z2 - g.ls2);
-  const float w = fmaf(g.ge, fmaf(z2, LN2, g.h - g.ls), g.gl);
-  return (c == g.label ? g.gl : 0.f) - p * w;
+  const bool own = c == g.label;
+  const float p = exp2_fast(z2 - (own ? g.ls2_y : g.ls2));
+  return (own ? g.g_y : 0.f) - p * fmaf(z2, g.w1, g.w0);
 }
 
 // Backward over strided classes: a thread has PV positions (bf16 two side by side, fp32 one) and `span` <= 64 classes, a
@@ -966,7 +987,7 @@ __global__ __launch_bounds__(256) void probs_bwd_rows(const BwdArgs<T> a, unsign
 }
 
 bool bad_positions(int64_t n0, int64_t n1, int64_t n2, int64_t classes, int64_t* n) {
-  if (n0 < 0 || n1 < 0 || n2 < 0 || classes <= 0 || classes > (1 << 30)) return true;
+  if (n0 < 0 || n1 < 0 || n2 < 0 || classes <= 0 || classes > MOST_CLASSES) return true;
   *n = n0 * n1 * n2;
   return *n > (1LL << 38);
 }
