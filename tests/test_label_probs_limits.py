@@ -1,0 +1,38 @@
+"""Sizes at the limits of the label-probability and gradient-norm C entries: what is refused, and what reaches the
+launch.  Addresses are made up, so these run only where there is no GPU to launch on."""
+import ctypes
+
+import pytest
+import torch
+
+from ldmseg.ops import native as K
+
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses must never be launched on")
+OK, ERR_ARG, ERR_LAUNCH = 0, 1, 3
+
+
+def _fwd(**kw):
+    p = K.LabelProbsParams(**{**dict(n0=1, n1=1, n2=4, s2=1, classes=5, sc=4, inner=1, temperature=1.0, dtype=0,
+                                     logits=16, entropy=16), **kw})
+    lib = K.load_library()
+    return lib.ldm_label_log_probs(ctypes.byref(p), None), lib.ldm_label_log_probs_workspace_bytes(ctypes.byref(p))
+
+
+def _bwd(**kw):
+    p = K.LabelProbsBwdParams(**{**dict(n0=1, n1=1, n2=4, s2=1, classes=5, sc=4, o2=1, oc=4, temperature=1.0, dtype=0,
+                                        logits=16, stats=16, d_logits=16), **kw})
+    return K.load_library().ldm_label_log_probs_bwd(ctypes.byref(p), None)
+
+
+@pytest.mark.parametrize("n", [
+    (1 << 32, 1 << 32, 1), (1 << 22, 1 << 22, 1 << 22), (3, 6148914691236517206, 1), (1, 1 << 62, 6), (1 << 39, 1, 1),
+    (1, 1 << 39, 1), (1 << 13, 1 << 13, 1 << 13)])
+def test_a_product_of_positions_past_64_bits_is_refused(n):
+    """2^32 x 2^32 is 0 in 64 bits and 3 x 6148914691236517206 is 2: neither is a call of that many positions."""
+    kw = dict(n0=n[0], n1=n[1], n2=n[2])
+    for layout in (dict(), dict(sc=1, s2=600, classes=600, oc=1, o2=600), dict(sc=1, s2=70000, classes=70000, oc=1, o2=70000)):
+        fwd = {k: v for k, v in layout.items() if k not in ("oc", "o2")}
+        assert _fwd(**kw, **fwd) == (ERR_ARG, 0), layout
+        assert _bwd(**kw, **layout) == ERR_ARG, layout
+    assert _fwd()[0] == ERR_LAUNCH and _bwd() == ERR_LAUNCH          # what is accepted reaches the launch
+    assert _fwd(n0=0)[0] == OK and _bwd(n1=0) == OK

@@ -988,8 +988,7 @@ __global__ __launch_bounds__(256) void probs_bwd_rows(const BwdArgs<T> a, unsign
 
 bool bad_positions(int64_t n0, int64_t n1, int64_t n2, int64_t classes, int64_t* n) {
   if (n0 < 0 || n1 < 0 || n2 < 0 || classes <= 0 || classes > MOST_CLASSES) return true;
-  *n = n0 * n1 * n2;
-  return *n > (1LL << 38);
+  return __builtin_mul_overflow(n0, n1, n) || __builtin_mul_overflow(*n, n2, n) || *n > (1LL << 38);
 }
 
 // A launch has less than 2^32 threads, blocks of 256 here; a call that would need more is refused.
@@ -1165,8 +1164,8 @@ bool bad_temperature(float t) { return !(t >= 1e-4f && t <= 1e4f); }
 }  // namespace
 
 extern "C" size_t ldm_label_log_probs_workspace_bytes(const ldm_label_probs_params* p) {
-  if (!p || !long_rows(p) || p->n0 <= 0 || p->n1 <= 0 || p->n2 <= 0) return 0;
-  const int64_t n = p->n0 * p->n1 * p->n2;
+  int64_t n;
+  if (!p || !long_rows(p) || bad_positions(p->n0, p->n1, p->n2, p->classes, &n) || n == 0) return 0;
   const int segments = segments_of(n, p->classes, p->dtype);
   return segments == 1 ? 0 : (size_t)(n * segments) * (sizeof(Part) + sizeof(uint64_t) * (size_t)std::max(0, p->topk));
 }
