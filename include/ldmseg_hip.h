@@ -733,8 +733,9 @@ int ldm_adamw(float* param, const float* grad, float* exp_avg, float* exp_avg_sq
  * ldm_label_log_probs_bwd: d_logits = (d_log_prob * (onehot(label) - p) - d_entropy * p * (log p +
  * entropy)) / temperature, written at the out strides o0, o1, o2, oc (the row's masked classes and
  * empty rows: 0). d_log_prob / d_entropy fp32 over the positions, either may be NULL.
- * Limits (LDM_ERR_ARG above them): strided classes 2^32 positions and, backward, 2^21 classes; adjacent
- * classes 2^24 rows of more than 8192, 2^25 shorter ones, and, backward, 2^32 packs of 16 bytes. */
+ * Limits (LDM_ERR_ARG above them): strided classes 2^32 - 256 positions and, backward, 2^21 classes; adjacent
+ * classes 2^24 - 1 rows of more than 8192, 2^25 - 4 shorter ones, and, backward, 2^24 - 1 runs of 4 KB (a
+ * row of 4 KB or more begins a run; shorter ones lie side by side in packs of 16 bytes). */
 #define LDM_LABEL_TOPK_MAX 16
 typedef struct {
   const void* logits;

@@ -140,3 +140,25 @@ def test_gradient_of_a_confident_label_keeps_its_digits(layout, T, dtype):
         if e is None:
             assert ((got.double().sum(-1)).abs() <= tol.sum(-1)).all()
             assert (got[own] != 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("C,N,masked", [(600_000, 32, False), (600_000, 3, True), (1 << 21, 2, False), (530_000, 70, True)])
+def test_gradient_of_many_strided_classes(C, N, masked, dtype):
+    """More classes than 65535 spans of 8, for fewer positions than a wave: the backward takes what the forward does."""
+    g = torch.Generator(device=DEV).manual_seed(C)
+    x = (torch.randn(1, C, N, device=DEV, generator=g) * 3)
+    x[0, C - 1, 0] = x[0, 5, 0] = 30.0
+    x = x.to(DT[dtype])
+    y = torch.randint(0, C, (1, N), device=DEV, generator=g)
+    y[0, 0] = C - 1
+    mask = None
+    if masked:
+        mask = torch.rand(1, C, device=DEV, generator=g) < 0.7
+        mask[0, y[0]] = True
+    gl, ge = (torch.randn(1, N, device=DEV, generator=g) for _ in range(2))
+    out, row = _check_forward(x, y, 1, 2, mask)
+    d = K.label_log_probs_bwd(x, out.stats, gl, ge, class_mask=mask)
+    want, tol = row.grad(y, gl.double(), ge.double(), x.dtype)
+    within(d.movedim(1, -1), want, tol, "gradient")
+    assert mask is None or (d[0, ~mask[0]] == 0).all()

@@ -36,3 +36,38 @@ def test_a_product_of_positions_past_64_bits_is_refused(n):
         assert _bwd(**kw, **layout) == ERR_ARG, layout
     assert _fwd()[0] == ERR_LAUNCH and _bwd() == ERR_LAUNCH          # what is accepted reaches the launch
     assert _fwd(n0=0)[0] == OK and _bwd(n1=0) == OK
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n", [1, 2, 32, 63, 64, 127, 128, 100_000])
+@pytest.mark.parametrize("classes", [16, 524_280, 524_281, 600_000, 1 << 20, (1 << 21) - 1, 1 << 21])
+def test_the_backward_takes_the_strided_classes_that_the_forward_takes(classes, n, dtype):
+    kw = dict(n2=n, classes=classes, sc=n + 1, dtype=dtype)
+    assert _fwd(**kw)[0] == ERR_LAUNCH
+    assert _bwd(**kw, oc=n + 1) == ERR_LAUNCH
+    mask = dict(class_mask=16, mask_stride=classes, mask_div=n)
+    assert _bwd(**kw, **mask, oc=n + 1) == ERR_LAUNCH
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_the_documented_limits(dtype):
+    """At the limit a call reaches the launch, one more is refused."""
+    def rows(classes, n):
+        kw = dict(n2=n, classes=classes, sc=1, s2=classes, dtype=dtype, workspace=16, workspace_bytes=1 << 40)
+        return _fwd(**kw)[0]
+
+    def rows_bwd(classes, n):
+        return _bwd(n2=n, classes=classes, sc=1, s2=classes, oc=1, o2=classes, dtype=dtype)
+
+    top = (1 << 32) - 256
+    planes = dict(classes=5, s2=5, sc=2, dtype=dtype)
+    assert _fwd(n2=top, **planes)[0] == ERR_LAUNCH and _fwd(n2=top + 1, **planes)[0] == ERR_ARG
+    assert _bwd(n2=top, o2=5, oc=2, **planes) == ERR_LAUNCH and _bwd(n2=top + 1, o2=5, oc=2, **planes) == ERR_ARG
+    for n in (1, 64, 100_000):
+        assert _bwd(n2=n, classes=(1 << 21) + 1, sc=n + 1, oc=n + 1, dtype=dtype) == ERR_ARG
+    assert rows(8193, (1 << 24) - 1) == ERR_LAUNCH and rows(8193, 1 << 24) == ERR_ARG
+    for classes in (8, 100, 1024, 1025, 8192):
+        assert rows(classes, (1 << 25) - 4) == ERR_LAUNCH
+    run = 4096 // (2 if dtype else 4)
+    assert rows_bwd(run, (1 << 24) - 1) == ERR_LAUNCH and rows_bwd(run, 1 << 24) == ERR_ARG
+    assert rows_bwd(run // 256, top) == ERR_LAUNCH and rows_bwd(run // 256, top + 1) == ERR_ARG

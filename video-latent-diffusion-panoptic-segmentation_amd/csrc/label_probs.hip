@@ -993,6 +993,7 @@ bool bad_positions(int64_t n0, int64_t n1, int64_t n2, int64_t classes, int64_t*
 
 // A launch has less than 2^32 threads, blocks of 256 here; a call that would need more is refused.
 constexpr int64_t MOST_BLOCKS = (1LL << 24) - 1;
+constexpr int MOST_SPANS = 65535, MOST_BWD_CLASSES = 1 << 21;
 
 // whether whole blocks of positions can share a row of the class mask, and the runs then
 bool mask_runs(const void* mask, int64_t mask_div, int64_t positions, int per_block, Tiling* t, int64_t* rows) {
@@ -1102,11 +1103,14 @@ int launch(const Args& a, void* ws, hipStream_t s) {
 
 template <typename T, int PV>
 int launch_bwd_planes(const BwdArgs<T>& a, int64_t n, hipStream_t s) {
-  // 32 classes to a thread, or down to 8 where the card would have less than 12 waves a CU
-  int span = 32;
-  while (span > 8 && n / 64 / PV * ((a.classes + span - 1) / span) < 12 * 256) span /= 2;
-  const unsigned spans = (unsigned)((a.classes + span - 1) / span);
-  if (spans > 65535 || (n + 255) / 256 > MOST_BLOCKS) return LDM_ERR_ARG;
+  if (a.classes > MOST_BWD_CLASSES || (n + 255) / 256 > MOST_BLOCKS) return LDM_ERR_ARG;
+  // 32 classes to a thread, or down to 8 where the card would have less than 12 waves a CU; no more spans than a grid has
+  // in y
+  const int64_t waves = (n + 64 * PV - 1) / (64 * PV);
+  auto spans_of = [&](int span) { return (a.classes + span - 1) / span; };
+  int span = spans_of(32) > MOST_SPANS ? 64 : 32;
+  while (span > 8 && waves * spans_of(span) < 12 * 256 && spans_of(span / 2) <= MOST_SPANS) span /= 2;
+  const unsigned spans = (unsigned)spans_of(span);
   Tiling t;
   int64_t rows;
   if (mask_runs(a.mask, a.mask_div, n, 256 * PV, &t, &rows)) {
