@@ -344,17 +344,17 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   numel.reserve(given);
   codes.reserve(given);
   std::vector<at::Tensor> keep;    // gradients stay alive until the launches are queued
-  keep.reserve(of_params ? given : 0);
+  keep.reserve(given);
   at::Device device(at::kCPU);
   at::TensorOptions options;
   for (Py_ssize_t i = 0; i < given; ++i) {
     const at::Tensor& t = tensor_of(PySequence_Fast_GET_ITEM(items, i), "a parameter");
-    if (of_params) {
-      at::Tensor g = t.grad();
-      if (!g.defined()) continue;
-      keep.push_back(std::move(g));
+    keep.push_back(of_params ? t.grad() : t);
+    if (!keep.back().defined()) {
+      keep.pop_back();
+      continue;
     }
-    const at::Tensor& g = of_params ? keep.back() : t;
+    const at::Tensor& g = keep.back();
     TORCH_CHECK_TYPE(g.layout() == at::kStrided, "sparse gradients are not supported");
     codes.push_back((uint8_t)dtype_code(g, "gradient dtype"));
     if (ptrs.empty()) {
@@ -364,7 +364,8 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     TORCH_CHECK_VALUE(g.device() == device, "gradients on ", device, " and ", g.device(), ": one device per call");
     TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense() || g.numel() == 0,
                       "a gradient is no dense memory (an expanded or strided view): make it contiguous");
-    if (clip) g.unsafeGetTensorImpl()->bump_version();       // written in place: autograd sees it
+    TORCH_CHECK(!clip || !g.is_inference() || c10::InferenceMode::is_enabled(),
+                "a gradient is an inference tensor: it can be clipped in inference mode only");
     numel.push_back(g.numel());
     ptrs.push_back(g.numel() ? g.data_ptr() : nullptr);
   }
@@ -382,6 +383,8 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   TORCH_CHECK_VALUE(rc != LDM_ERR_OVERLAP,
                     "gradients overlap in memory (the same gradient twice, or views of one another)");
   check_status(rc, "ldm_grad_norm");
+  if (clip)                        // written in place: autograd sees it.  A refused call has not come here
+    for (const at::Tensor& g : keep) g.unsafeGetTensorImpl()->bump_version();
   if (clip || args[5] != Py_None) return THPVariable_Wrap(out.select(0, 0));
   return Py_BuildValue("NN", THPVariable_Wrap(out.select(0, 0)), THPVariable_Wrap(out));
   END_HANDLE_TH_ERRORS
