@@ -1,6 +1,7 @@
 """``label_log_probs`` as an autograd node: log probabilities of given labels and entropies of every position of
 class logits, differentiable in the logits, with the most likely alternatives (ops.native has the launches)."""
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import native as K
@@ -30,11 +31,14 @@ class _LabelLogProbs(torch.autograd.Function):
 
 def label_log_probs(logits, labels=None, *, dim=1, topk=0, temperature=1.0, ignore_label=None, class_mask=None):
     """ops.native.label_log_probs with gradients: ``log_prob`` and ``entropy`` of the result are differentiable
-    in ``logits`` (the alternatives are not).  Without a gradient to take it saves nothing for one.
+    in ``logits`` (the alternatives are not), backward and once.  Without a gradient to take it saves nothing for one.
 
         nll = -label_log_probs(logits, labels, ignore_label=255).log_prob.sum() / (labels != 255).sum()
         nll.backward()
     """
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise NotImplementedError("label_log_probs has no forward-mode derivative: take its gradient backward, or call "
+                                  "it on logits without a tangent")
     if torch.is_grad_enabled() and logits.requires_grad:
         return K.LabelProbs(*_LabelLogProbs.apply(logits, labels, dim, topk, temperature, ignore_label, class_mask),
                             None)
