@@ -207,8 +207,8 @@ _lock = threading.Lock()
 
 def load_library(path=None):
     """Load the HIP library (no GPU needed to load it; kernels need one to run).  The env variable
-    LDMSEG_HIP_LIB selects another build of it (A/B runs of an ablation or older build: entries
-    that it lacks are skipped, and a call of one fails)."""
+    LDMSEG_HIP_LIB selects another build of it (A/B runs of an ablation or older build, whose
+    tuning hooks may be missing: only those are then skipped)."""
     global _lib
     override = path is not None or bool(os.environ.get("LDMSEG_HIP_LIB"))
     path = path or os.environ.get("LDMSEG_HIP_LIB") or LIB_PATH
@@ -220,7 +220,7 @@ def load_library(path=None):
                                    f"(or __graft_entry__.build()) first")
             lib = ctypes.CDLL(path)
             for name, (res, args) in EXPORTS.items():
-                if override and not hasattr(lib, name):
+                if override and not hasattr(lib, name) and ("_set_" in name or "describe" in name):
                     continue
                 fn = getattr(lib, name)
                 fn.restype = res
