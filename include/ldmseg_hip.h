@@ -776,6 +776,7 @@ int ldm_label_log_probs_bwd(const ldm_label_probs_bwd_params* p, ldm_stream_t st
  *                         (LDM_F32 / LDM_BF16, mixed freely); each tensor is dense memory, aligned
  *                         to its element; tensors must not overlap (LDM_ERR_OVERLAP).  The arrays are
  *                         read during the call only: a captured graph keeps its own copy.
+ *                         2^46 values in all (LDM_ERR_ARG above).
  *   norm_type             LDM_NORM_2 (sqrt of the fp64 sum of squares), LDM_NORM_INF, LDM_NORM_1
  *   out                   device fp32 [2]: the norm and the factor min(1, max_norm / (norm + 1e-6))
  *   clip                  0: norm only.  1: norm, then every g *= factor where the factor is below

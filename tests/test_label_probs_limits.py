@@ -71,3 +71,20 @@ def test_the_documented_limits(dtype):
     run = 4096 // (2 if dtype else 4)
     assert rows_bwd(run, (1 << 24) - 1) == ERR_LAUNCH and rows_bwd(run, 1 << 24) == ERR_ARG
     assert rows_bwd(run // 256, top) == ERR_LAUNCH and rows_bwd(run // 256, top + 1) == ERR_ARG
+
+
+@pytest.mark.parametrize("code", [0, 1])
+@pytest.mark.parametrize("numel", [[1 << 62], [(1 << 62) + 5], [(1 << 63) - 1], [1 << 61, 7], [(1 << 46) + 1],
+                                   [1 << 45] * 3, [16, (1 << 63) - 8, 16]])
+def test_gradients_past_the_address_space_are_refused(numel, code):
+    """2^62 fp32 values are 0 bytes in 64 bits and 2^62 + 5 are 20: a clip of them must not answer that all is well."""
+    lib = K.load_library()
+    n = len(numel)
+    sizes, codes = (ctypes.c_int64 * n)(*numel), bytes([code]) * n
+    ptrs = (ctypes.c_uint64 * n)(*[4096 + (i << 55) for i in range(n)])
+    assert lib.ldm_grad_norm_workspace_bytes(sizes, n) == 0
+    for clip in (0, 1, 2):
+        assert lib.ldm_grad_norm(ptrs, sizes, codes, n, 0, 1.0, clip, 64, 64, 1 << 62, None) == ERR_ARG
+    # an address and a size whose end passes the largest address
+    ends = (ctypes.c_uint64 * 1)((1 << 63) - 64)
+    assert lib.ldm_grad_norm(ends, (ctypes.c_int64 * 1)(1 << 20), bytes([code]), 1, 0, 1.0, 1, 64, 64, 1 << 62, None) == ERR_ARG

@@ -304,6 +304,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void clip_small(const SmallTable 
 
 // a span above 2^30 elements is listed in pieces (of whole chunks)
 constexpr int64_t PIECE = 1LL << 30;
+// Values of a call at most: no sum of sizes or addresses below leaves 64 bits
+constexpr int64_t MOST_VALUES = 1LL << 46;
 int64_t entries_of(const int64_t* numel, int n) {
   int64_t c = 0;
   for (int i = 0; i < n; ++i) c += (numel[i] + PIECE - 1) / PIECE;
@@ -355,6 +357,7 @@ extern "C" size_t ldm_grad_norm_workspace_bytes(const int64_t* numel, int ntenso
   int64_t total = 0, small = 0, large = 0, units = 0;
   for (int i = 0; i < ntensors; ++i)
     if (numel[i] > 0) {
+      if (numel[i] > MOST_VALUES - total) return 0;                           // ldm_grad_norm refuses it
       total += numel[i];
       units += (numel[i] * 4 + 1023) / 1024;
       small += (numel[i] + chunk_of<float, SMALL_PACKS>() - 1) / chunk_of<float, SMALL_PACKS>();
@@ -415,12 +418,15 @@ extern "C" int ldm_grad_norm(const void* const* ptrs, const int64_t* numel, cons
   try {
     std::vector<Span> spans;
     spans.reserve(ntensors);
+    int64_t total = 0;
     for (int i = 0; i < ntensors; ++i) {
       if (numel[i] < 0 || dtypes[i] > LDM_BF16) return LDM_ERR_ARG;
       if (numel[i] == 0) continue;
       const uint64_t a = reinterpret_cast<uint64_t>(ptrs[i]);
       const uint64_t size = dtypes[i] == LDM_BF16 ? 2 : 4;
-      if (!a || (a >> 63)) return LDM_ERR_ARG;
+      if (numel[i] > MOST_VALUES - total) return LDM_ERR_ARG;
+      total += numel[i];
+      if (!a || (a >> 63) || ((a + size * (uint64_t)numel[i]) >> 63)) return LDM_ERR_ARG;
       if (a % size) return LDM_ERR_ALIGN;
       spans.push_back({a, a + size * (uint64_t)numel[i], size});
     }
