@@ -162,3 +162,26 @@ def test_gradient_of_many_strided_classes(C, N, masked, dtype):
     want, tol = row.grad(y, gl.double(), ge.double(), x.dtype)
     within(d.movedim(1, -1), want, tol, "gradient")
     assert mask is None or (d[0, ~mask[0]] == 0).all()
+
+
+def test_lazily_negated_tensors_are_read_as_they_are():
+    """The imaginary part of a conjugate is a view that torch negates as it reads: logits and arriving gradients of that
+    kind have their own sign."""
+    g = torch.Generator().manual_seed(7)
+
+    def view(*shape):
+        v = torch.complex(torch.randn(*shape, generator=g), torch.randn(*shape, generator=g)).to(DEV).conj().imag
+        assert v.is_neg()
+        return v
+
+    for shape in ((2, 19, 33), (40, 300), (1, 7, 1)):
+        x, y = view(*shape), torch.randint(0, shape[1], shape[:1] + shape[2:], generator=g).to(DEV)
+        gl, ge = view(*y.shape), view(*y.shape)
+        out, ref = (K.label_log_probs(v, y, topk=3, want_stats=True) for v in (x, x.resolve_neg().contiguous()))
+        assert torch.equal(out.top_ids, ref.top_ids)
+        assert (out.log_prob - ref.log_prob).abs().max() < 1e-5 and (out.entropy - ref.entropy).abs().max() < 1e-5
+        d = K.label_log_probs_bwd(x, out.stats, gl, ge)
+        want = K.label_log_probs_bwd(x.resolve_neg().contiguous(), ref.stats, gl.resolve_neg(), ge.resolve_neg())
+        assert (d - want).abs().max() < 1e-5
+    one = torch._neg_view(torch.randn(1, 5, 1, generator=g).to(DEV))
+    assert torch.equal(K.label_log_probs(one).entropy, K.label_log_probs(one.resolve_neg()).entropy)

@@ -123,6 +123,9 @@ Positions positions_of(const at::Tensor& x, int64_t dim, bool with_out) {
   }
 }
 
+// what a lazily negated view shows, not what its memory holds
+at::Tensor logits_of(PyObject* o) { return tensor_of(o, "logits").resolve_neg(); }
+
 int64_t class_dim(const at::Tensor& logits, int64_t dim) {
   const int64_t nd = logits.dim();
   TORCH_CHECK_VALUE(nd >= 2, "logits need a class dim and at least one position dim");
@@ -174,7 +177,7 @@ PyObject* wrap_or_none(const at::Tensor& t) {
 PyObject* label_log_probs(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   TORCH_CHECK(nargs == 8 && p_fwd, "label_log_probs: 8 arguments after init()");
-  const at::Tensor& logits = tensor_of(args[0], "logits");
+  const at::Tensor logits = logits_of(args[0]);
   const int code = dtype_code(logits, "dtype");
   const int64_t dim = class_dim(logits, int_of(args[2], "dim"));
   const int64_t topk = int_of(args[3], "topk"), C = logits.size(dim);
@@ -261,14 +264,14 @@ at::Tensor upstream(PyObject* o, const at::DimVector& shape, const at::Tensor& l
   TORCH_CHECK_VALUE(g.scalar_type() == at::kFloat && g.device() == logits.device() &&
                     g.sizes() == at::IntArrayRef(shape), name, " must be fp32 ", at::IntArrayRef(shape),
                     " on the logits' device");
-  return g.contiguous();
+  return g.resolve_neg().contiguous();
 }
 
 // (logits, stats, d_log_prob | None, d_entropy | None, dim, temperature, class_mask | None) -> d_logits
 PyObject* label_log_probs_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   TORCH_CHECK(nargs == 7 && p_bwd, "label_log_probs_bwd: 7 arguments after init()");
-  const at::Tensor& logits = tensor_of(args[0], "logits");
+  const at::Tensor logits = logits_of(args[0]);
   const int code = dtype_code(logits, "dtype");
   const int64_t dim = class_dim(logits, int_of(args[4], "dim"));
   const float temperature = temperature_of(args[5]);
