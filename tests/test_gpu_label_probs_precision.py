@@ -185,3 +185,65 @@ def test_lazily_negated_tensors_are_read_as_they_are():
         assert (d - want).abs().max() < 1e-5
     one = torch._neg_view(torch.randn(1, 5, 1, generator=g).to(DEV))
     assert torch.equal(K.label_log_probs(one).entropy, K.label_log_probs(one.resolve_neg()).entropy)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape,T,masked", [
+    ((5, 7), 1.0, False), ((513, 30), 1.0, True), ((3, 1023), 0.7, False), ((4, 1025), 1.0, False), ((70, 5000), 1.0, True),
+    ((70, 5000), 1.0, False), ((1, 16385), 1.0, False), ((3, 40001), 0.7, True), ((1, 131072), 1.0, False),
+    ((2051, 2001), 1.0, False), ((9, 2041), 1.0, False), ((300, 4099), 2.0, True),
+    ((2, 30, 24, 80), 1.0, False), ((1, 128, 37, 53), 1.0, True), ((2, 33, 17, 31), 0.7, False), ((1, 513, 3, 67), 1.0, False),
+    ((3, 19, 8, 8), 1.0, True), ((2, 70, 64, 66), 0.5, False),
+])
+def test_gradient_element_by_element(shape, T, masked, dtype):
+    """Every element against a bound of its own size: most are far below the largest of their row, and neither they nor a
+    row's last ones could be left out or swapped unseen."""
+    g = torch.Generator().manual_seed(sum(shape))
+    N, C = shape[:2]
+    x = (torch.randn(shape, generator=g) * 3).to(DT[dtype]).to(DEV)
+    y = torch.randint(0, C, shape[:1] + shape[2:], generator=g)
+    y = torch.where(torch.rand(y.shape, generator=g) < 0.3, x.argmax(1).cpu(), y).to(DEV)
+    mask = None
+    if masked:
+        mask = torch.rand(N, C, generator=g) < 0.7
+        mask[:, 0] = True
+        y = torch.where(mask.to(DEV).view(N, C, *[1] * (x.ndim - 2)).expand(x.shape).gather(1, y.unsqueeze(1))[:, 0], y, 0)
+        mask = mask.to(DEV)
+    gl, ge = (torch.randn(y.shape, generator=g).to(DEV) for _ in range(2))
+    out, row = _check_forward(x, y, 1, 0, mask, T)
+    for a, b in ((gl, None), (None, ge), (gl, ge)):
+        got = K.label_log_probs_bwd(x, out.stats, a, b, temperature=T, class_mask=mask).movedim(1, -1)
+        want, tol = row.grad(y, a if a is None else a.double(), b if b is None else b.double(), x.dtype)
+        if masked:
+            left = mask.view(N, *[1] * (x.ndim - 2), C).expand(want.shape)
+            assert (got[~left] == 0).all()
+        else:
+            left = torch.ones_like(want, dtype=torch.bool)
+        # the bound tells: twice it is less than the element, nearly everywhere and in the last classes too
+        tells = (2 * tol < want.abs()) | ~left
+        assert tells.double().mean() > 0.9 and tells[..., -16:].double().mean() > 0.9
+        within(got, want, tol, "gradient")
+
+
+def test_rows_past_32_bits_of_elements():
+    """2.2e6 rows of 1000 bf16 classes in a matrix of 2.2e9 elements: both ends, forward and backward."""
+    if torch.cuda.get_device_properties(0).total_memory < 40e9:
+        pytest.skip("needs 20 GB")
+    g = torch.Generator().manual_seed(3)
+    N, C = 2_200_000, 1000
+    x = torch.zeros(N, C + 1, dtype=torch.bfloat16, device=DEV)[:, :C]
+    ends = torch.tensor([0, 1, N // 2, N - 3, N - 2, N - 1], device=DEV)
+    x[ends[1:]] = torch.randn(5, C, generator=g).bfloat16().to(DEV)
+    y = torch.zeros(N, dtype=torch.int64, device=DEV)
+    y[ends] = torch.tensor([3, 999, 17, 0, 501, 998], device=DEV)
+    out = K.label_log_probs(x, y, topk=2, want_stats=True)
+    row, ids = Row(x[ends]), y[ends, None]
+    within(out.entropy[ends], row.H, row.err_H(), "entropy")
+    within(out.log_prob[ends, None], row.log_p(ids), row.err_log_p(ids), "log_prob")
+    assert abs(out.log_prob[0].item() + math.log(C)) < 1e-4 and abs(out.log_prob[5].item() + math.log(C)) < 1e-4
+    assert torch.equal(out.top_ids[ends[1:]].long(), x[ends[1:]].float().topk(2, dim=1).indices)
+    gl = torch.ones(N, device=DEV)
+    gl[ends] = torch.randn(6, generator=g).to(DEV)
+    d = K.label_log_probs_bwd(x, out.stats, gl)
+    want, tol = row.grad(y[ends], gl[ends].double(), None, x.dtype)
+    within(d[ends], want, tol, "gradient")
