@@ -326,6 +326,26 @@ PyObject* label_positions(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // ------------------------------------------------------------------------------------ gradient norms
+// The first n tensors of a list, or of a sequence, marked as modified while it is walked, unless what follows throws
+// (in a walk of its own after the launches 700 gradients cost the host 20 us for 16, waiting for version counters).
+struct Marks {
+  const std::vector<at::Tensor>& list;
+  PyObject* sequence;              // or null
+  size_t n = 0;
+  void add(const at::Tensor& t) {
+    t.unsafeGetTensorImpl()->bump_version();       // throws at an inference tensor outside inference mode
+    ++n;
+  }
+  ~Marks() {
+    for (size_t i = 0; i < n; ++i) {
+      const at::Tensor& t = sequence ? THPVariable_Unpack(PySequence_Fast_GET_ITEM(sequence, i)) : list[i];
+      if (t.unsafeGetTensorImpl()->is_inference()) continue;               // has no version
+      c10::VariableVersion v = t.unsafeGetTensorImpl()->version_counter();
+      v.set_version((int64_t)v.current_version() - 1);
+    }
+  }
+};
+
 // (tensors, of_params, norm_type code, max_norm, clip, out | None): the norm and the factor of `tensors` (or, with
 // of_params, of the gradients that they have), clip as in ldm_grad_norm -> the norm, or (norm, out) where clip is 0
 // and out None; None without a gradient
@@ -347,17 +367,18 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   numel.reserve(given);
   codes.reserve(given);
   std::vector<at::Tensor> keep;    // gradients stay alive until the launches are queued
-  keep.reserve(given);
+  keep.reserve(of_params ? given : 0);
+  Marks marks{keep, of_params ? nullptr : items};
   at::Device device(at::kCPU);
   at::TensorOptions options;
   for (Py_ssize_t i = 0; i < given; ++i) {
     const at::Tensor& t = tensor_of(PySequence_Fast_GET_ITEM(items, i), "a parameter");
-    keep.push_back(of_params ? t.grad() : t);
-    if (!keep.back().defined()) {
-      keep.pop_back();
-      continue;
+    if (of_params) {
+      at::Tensor g = t.grad();
+      if (!g.defined()) continue;
+      keep.push_back(std::move(g));
     }
-    const at::Tensor& g = keep.back();
+    const at::Tensor& g = of_params ? keep.back() : t;
     TORCH_CHECK_TYPE(g.layout() == at::kStrided, "sparse gradients are not supported");
     codes.push_back((uint8_t)dtype_code(g, "gradient dtype"));
     if (ptrs.empty()) {
@@ -367,8 +388,7 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     TORCH_CHECK_VALUE(g.device() == device, "gradients on ", device, " and ", g.device(), ": one device per call");
     TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense() || g.numel() == 0,
                       "a gradient is no dense memory (an expanded or strided view): make it contiguous");
-    TORCH_CHECK(!clip || !g.is_inference() || c10::InferenceMode::is_enabled(),
-                "a gradient is an inference tensor: it can be clipped in inference mode only");
+    if (clip) marks.add(g);        // written in place: autograd sees it
     numel.push_back(g.numel());
     ptrs.push_back(g.numel() ? g.data_ptr() : nullptr);
   }
@@ -386,8 +406,7 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   TORCH_CHECK_VALUE(rc != LDM_ERR_OVERLAP,
                     "gradients overlap in memory (the same gradient twice, or views of one another)");
   check_status(rc, "ldm_grad_norm");
-  if (clip)                        // written in place: autograd sees it.  A refused call has not come here
-    for (const at::Tensor& g : keep) g.unsafeGetTensorImpl()->bump_version();
+  marks.n = 0;                     // a refused call has not come here: its marks are taken back
   if (clip || args[5] != Py_None) return THPVariable_Wrap(out.select(0, 0));
   return Py_BuildValue("NN", THPVariable_Wrap(out.select(0, 0)), THPVariable_Wrap(out));
   END_HANDLE_TH_ERRORS
