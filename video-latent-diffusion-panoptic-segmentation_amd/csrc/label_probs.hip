@@ -10,11 +10,12 @@
 // cancels where 1 - p is small.  Backward, from the saved m, log1p(r) and entropy:
 //   p_j = exp((x_j - m) / T - log1p(r))
 //   d x_j = (g_l (1[j == y] - p_j) - g_H p_j (log p_j + H)) / T
-// All sums are fp32; the logits are exact in fp32 and d x_j is rounded once to their type.
+// Sums are fp32 over at most 512 logits of a thread and fp64 beyond; the logits are exact in fp32 and d x_j is rounded
+// once to their type.
 // The logits are read once each way and the gradient written once: memory bounds the fp32 kernels (copies reach 5.3
 // TB/s here), the vector pipe the bf16 ones, whose 13 instructions and one exp a class take about as long as 2 bytes.
-// exp is the hardware's exp2 of one rounded product, so a term e^z carries a relative error of
-// about |z| 2^-24: at most 0.37 x 2^-24 of the largest term.
+// exp is the hardware's exp2 of a product: x - m, log2(e) / T, their product and exp2 round, so a term e^z carries a
+// relative error of at most (4 |z| + 5) 2^-24, which is no more than 5 x 2^-24 of the largest term.
 #include "common.h"
 
 #include <algorithm>
@@ -295,7 +296,7 @@ __device__ __forceinline__ void store_row(const Args& a, int64_t pos, const Soft
 
 // Short rows of adjacent classes: G lanes to a row, E packs of VEC classes to a lane (16 classes), all of it in
 // registers.  A row's last pack reaches back over its neighbour; the classes it has in common with it count once.
-// 32768 x 30 bf16 with 3 alternatives: 6.0 us, the latency of one launch, load, reduction and store.
+// 32768 x 30 bf16 with 3 alternatives: 5.2 us, the latency of one launch, load, reduction and store.
 template <typename T, int VEC, int G, int E, bool TOP>
 __global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
   constexpr int N = VEC * E;
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(256) void probs_short_rows(const Args a) {
 // in flight.  One segment to a row: the block finishes it.  More: what the segments come to goes to the workspace
 // and probs_join finishes the row.  4096 x 16384 fp32: 57 us (4.7 TB/s), bf16 31 us back to back (4.3 TB/s, the vector pipe), 38
 // one at a time; four packs in flight: 55 and 31, but rows of 4096 took 68 us for 44.  One row of 65537 fp32: 6 us in 65 segments, with 8
-// alternatives 12 us, half of it in each launch.
+// alternatives 12 us, 7 in the first launch and 5 in the second.
 struct Part { float m, r, t; int nan; };
 // (key, class) as one number: larger is earlier in the answer (larger key, then lower class), 0 is none
 __device__ __forceinline__ uint64_t candidate(int key, int id) {
@@ -642,7 +643,7 @@ __global__ __launch_bounds__(256) void probs_join(const Args a, int segments, co
 
 // What a thread of probs_planes keeps of the most likely classes of one position: values in falling order.  A new
 // value's place is the median of its neighbours (v_med3); a later class needs a larger value.  NaNs are sorted out
-// afterwards (nan_first): here they compare false.
+// afterwards, from the position's logits: here they compare false.
 template <int K>
 struct TopValues {
   float v[K > 0 ? K : 1];
@@ -718,7 +719,7 @@ constexpr int PLANES_UNR = 8;
 // Unsplit bf16 takes 16 classes at a time: as many bytes in flight as 8 of fp32, and half the rescales (8 x 128 x 256 x
 // 256: 36.4 us for 39.4); fp32 gains nothing by it and split calls lose 3 %.  Two positions a
 // thread: 42 us.
-// 1 x 400 x 40 x 50 fp32: 9.6 us split, 19.1 us not.
+// 1 x 400 x 40 x 50 fp32: 8.0 us split, 19.1 us not.
 template <typename T, int K, bool SPLIT, bool LISTED, bool FOLDS>
 __global__ __launch_bounds__(256) void probs_planes(const Args a, const Tiling tile) {
   constexpr int UNR = PLANES_UNR;
@@ -944,7 +945,7 @@ __global__ __launch_bounds__(256) void probs_bwd_planes(const BwdArgs<T> a, cons
 
 // Backward over adjacent classes: a thread has UN packs of VEC classes of one row; a row's last pack reaches back
 // over its neighbour and only its own classes are written.  FLAT: packs of short rows side by side in a block.
-// 4096 x 16384 bf16: 45 us (5.9 TB/s: the forward has left part of the logits in the memory-side cache).
+// 4096 x 16384 bf16: 44 us (6.1 TB/s: the forward has left part of the logits in the memory-side cache).
 template <typename T, int VEC, int UN, bool FLAT>
 __global__ __launch_bounds__(256) void probs_bwd_rows(const BwdArgs<T> a, unsigned per_row, unsigned blocks_per_row) {
   int64_t pos;
@@ -1144,7 +1145,7 @@ int launch_bwd(const ldm_label_probs_bwd_params* p, int64_t n, hipStream_t s) {
       hipLaunchKernelGGL((probs_bwd_rows<T, RV, 1, true>), dim3((unsigned)blocks), dim3(256), 0, s, a, per_row, 1u);
     } else {
       // two packs to a thread where that leaves little of the row's last block without one (3000 x 5892 bf16, 737 packs:
-      // 15.1 us with one, 18.6 us with two; 4096 x 16384, 2048 packs: 50 and 47 us)
+      // 14.7 us with one, 18.6 us with two; 4096 x 16384, 2048 packs: 47 and 44 us)
       const unsigned two = (per_row + 511) / 512;
       const bool full = per_row * 10 >= two * 512 * 9;
       const unsigned bpr = full ? two : (per_row + 255) / 256;
